@@ -314,6 +314,84 @@ MMC_EXPORT int mmc_op_attention_noalloc(int32_t batch, int32_t nq, int32_t nkv, 
  * slab: the cache's swizzled row layout, for tools that read pages directly. */
 MMC_EXPORT int64_t mmc_kv_row_offset(int32_t hd, int32_t row, int32_t chunk);
 
+/* ------------------------------------------------------------- low-bit ops
+ * The operators of a quantised attention block, beside the fp16 ones above:
+ * append and attention over a paged cache in 8 bits, and projections with
+ * weights in 4 bits. All pointers are device memory of the current device (16-byte aligned unless
+ * they are int32), launches are asynchronous on `stream` (NULL: the default
+ * stream) and may be captured into a graph. What the host can see is checked
+ * before anything is launched (MMC_ERR_INVALID); what lies in device memory the
+ * kernels check before use, and report in the cache's error word. */
+
+/* A paged KV cache in 8 bits: values are code * scale, codes e4m3 (1 sign, 4
+ * exponent, 3 mantissa bits, largest 448), scales powers of two, one for each 16
+ * positions of a page, kv head and K or V: the smallest 2^e (e >= -126) with
+ * |value| <= 448 * 2^e over the block's positions so far.
+ *   d_codes       [n_pages][layers][2 (K, V)][nkv][64][hd] bytes
+ *   d_scales      [n_pages][layers][2][nkv][4] fp32
+ *   d_block_table [max_seqs][max_pages] page of each 64 positions of a slot
+ *   d_seq_pos     [max_seqs] positions of a slot BEFORE a call's rows; not
+ *                 modified by the operators: advance it after the last layer
+ *   d_error       one int32, zeroed by the caller before its first use; kernels
+ *                 set it, mmc_op_kv8_status reads and clears it
+ * hd is 16, 32, 64, 96 or 128. A block whose positions hold an infinity or a NaN
+ * has the scale NaN, and so has every output that reads it.
+ *
+ * Batches: sequence i of a call has slot d_slots[i] and the rows
+ * d_row_start[i] .. d_row_start[i + 1] - 1 (n_seqs + 1 ascending int32; NULL:
+ * one row each, rows == n_seqs), at the positions d_seq_pos[slot] on. `rows` is
+ * the number of rows of the buffers, `max_new` the most rows of one sequence.
+ * A negative slot marks an unused sequence. Rows that belong to no sequence are
+ * neither read nor written. */
+typedef struct mmc_kv8_cache {
+  int32_t n_pages, layers, nkv, hd, max_seqs, max_pages;
+  void* d_codes;
+  float* d_scales;
+  const int32_t* d_block_table;
+  const int32_t* d_seq_pos;
+  int32_t* d_error;
+} mmc_kv8_cache;
+
+/* q/k RMSNorm (d_q_norm, d_k_norm [hd], both or neither) + RoPE of the raw
+ * projections d_qkv [rows][(nq + 2 nkv) * hd] fp32; q goes to d_q_fp16
+ * [rows][nq * hd], K and V into the cache. Older positions of a block whose
+ * scale grows go over to the new scale; positions behind the new ones are left
+ * as they were. d_rope_cos/sin [max_pos][hd / 2]. An unused sequence's rows of
+ * d_q are left as they were, and so are those of a sequence that is refused (a
+ * slot that appears twice with rows, rows or positions out of range). */
+MMC_EXPORT int mmc_op_kv8_append(const mmc_kv8_cache* cache, int32_t layer, int32_t n_seqs, int32_t rows,
+                                 int32_t max_new, const int32_t* d_slots, const int32_t* d_row_start, int32_t nq,
+                                 const float* d_qkv, const float* d_q_norm, const float* d_k_norm,
+                                 const float* d_rope_cos, const float* d_rope_sin, int32_t max_pos, float eps,
+                                 void* d_q_fp16, void* stream);
+/* Grouped-query attention of the call's rows over the cache, their own
+ * positions included (append first): row j of a sequence attends positions
+ * 0 .. d_seq_pos[slot] + j. d_out_fp16 [rows][nq * hd]; the rows of an unused
+ * sequence are zero, those of a sequence that is refused are left as they were.
+ * `max_ctx` bounds d_seq_pos + rows over the sequences (the workspace and the
+ * split of the work go by it). A workspace serves one call at a time: calls that
+ * may overlap on the GPU (other streams, graphs replayed side by side) need one
+ * each. Its contents need no preparation. */
+MMC_EXPORT int mmc_op_kv8_attention_workspace_size(const mmc_kv8_cache* cache, int32_t n_seqs, int32_t rows,
+                                                   int32_t max_new, int32_t nq, int32_t max_ctx, size_t* bytes);
+MMC_EXPORT int mmc_op_kv8_attention(const mmc_kv8_cache* cache, int32_t layer, int32_t n_seqs, int32_t rows,
+                                    int32_t max_new, const int32_t* d_slots, const int32_t* d_row_start, int32_t nq,
+                                    const void* d_q_fp16, int32_t max_ctx, void* d_out_fp16, void* d_workspace,
+                                    size_t workspace_bytes, void* stream);
+/* Waits for `stream` and reports the cache's error word: MMC_ERR_DEVICE with the
+ * reason if a kernel set it (which also clears it). Not during a capture. */
+MMC_EXPORT int mmc_op_kv8_status(const mmc_kv8_cache* cache, void* stream);
+
+/* y[b][n] = sum_k (c[n][k] - z[n][k / group]) * s[n][k / group] * x[b][k].
+ *   d_codes   [n][k / 2] bytes, column 2i in the low four bits of byte i
+ *   d_scales  [n][k / group] fp16
+ *   d_zeros   [n][k / group] bytes (0..15 in use, any value is taken), or NULL: 8
+ *   d_x       [batch][k] fp16, d_y [batch][n] fp32
+ * group is 32, 64 or 128 and divides k. Products and sums are exact or fp32. */
+MMC_EXPORT int mmc_op_w4_projection(int32_t batch, int32_t n, int32_t k, int32_t group, const void* d_codes,
+                                    const void* d_scales_fp16, const void* d_zeros, const void* d_x_fp16, float* d_y,
+                                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

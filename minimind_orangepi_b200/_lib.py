@@ -38,6 +38,23 @@ class ModelDesc(C.Structure):
     ]
 
 
+class Kv8Cache(C.Structure):
+    """mmc_kv8_cache: a paged KV cache in 8 bits (device pointers as integers)."""
+    _fields_ = [
+        ("n_pages", C.c_int32),
+        ("layers", C.c_int32),
+        ("nkv", C.c_int32),
+        ("hd", C.c_int32),
+        ("max_seqs", C.c_int32),
+        ("max_pages", C.c_int32),
+        ("d_codes", C.c_void_p),
+        ("d_scales", C.c_void_p),
+        ("d_block_table", C.c_void_p),
+        ("d_seq_pos", C.c_void_p),
+        ("d_error", C.c_void_p),
+    ]
+
+
 EXPORTS = {
     # name: (restype, argtypes)
     "mmc_last_error": (C.c_char_p, []),
@@ -90,6 +107,17 @@ EXPORTS = {
                                            C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32,
                                            C.c_float, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p,
                                            C.c_int32, C.c_void_p, C.c_void_p]),
+    "mmc_op_kv8_append": (C.c_int, [C.POINTER(Kv8Cache), C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p,
+                                    C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                    C.c_void_p, C.c_int32, C.c_float, C.c_void_p, C.c_void_p]),
+    "mmc_op_kv8_attention_workspace_size": (C.c_int, [C.POINTER(Kv8Cache), C.c_int32, C.c_int32, C.c_int32,
+                                                      C.c_int32, C.c_int32, C.POINTER(C.c_size_t)]),
+    "mmc_op_kv8_attention": (C.c_int, [C.POINTER(Kv8Cache), C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p,
+                                       C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p,
+                                       C.c_size_t, C.c_void_p]),
+    "mmc_op_kv8_status": (C.c_int, [C.POINTER(Kv8Cache), C.c_void_p]),
+    "mmc_op_w4_projection": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p,
+                                       C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "mmc_kv_row_offset": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32]),
 }
 

@@ -40,8 +40,11 @@ CUDA_SOURCES = [
     CSRC / "kernels" / "pack.cu",
     CSRC / "kernels" / "step_kernel.cu",
     CSRC / "kernels" / "skinny.cu",
+    CSRC / "kernels" / "kv8.cu",
+    CSRC / "kernels" / "w4.cu",
     CSRC / "mmc_api.cu",
     CSRC / "attention_noalloc.cu",
+    CSRC / "lowbit_api.cu",
 ]
 RUNTIME_SOURCES = [
     CSRC / "runtime" / "config.cpp",

@@ -1,0 +1,608 @@
+"""The low-bit operators against their 64-bit forms, through the C ABI: append and
+attention over the 8-bit paged cache, 4-bit projections, and a run of them
+together. The tolerances are derived where they are computed."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import pytest
+
+from minimind_orangepi_b200._lib import Kv8Cache, check, lib
+
+torch = pytest.importorskip("torch")
+
+from lowbit_reference import Cache, PAGE, attention, e4m3_table, norm_rope, w4_weights  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+EPS = 1e-5
+DEVICE_ERROR = 5
+
+
+def ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+class World:
+    """A cache with random contents in every position, a table of shuffled pages, and the batch of one call."""
+
+    def __init__(self, seed, nq, nkv, hd, pos, new, layers=1, layer=0, spare_rows=0, unused=(), size=1.0):
+        g = self.g = torch.Generator().manual_seed(seed)
+        self.nq, self.nkv, self.hd, self.layers, self.layer = nq, nkv, hd, layers, layer
+        self.pos, self.new, self.seqs, self.unused = pos, new, len(pos), set(unused)
+        need = [max(1, -(-(p + n) // PAGE)) for p, n in zip(pos, new)]
+        self.n_pages, self.max_pages, self.max_seqs = sum(need) + 2, max(need) + 1, self.seqs + 2
+        order = torch.randperm(self.n_pages, generator=g).tolist()
+        self.slots = torch.randperm(self.max_seqs, generator=g)[:self.seqs].tolist()
+        self.table = torch.full((self.max_seqs, self.max_pages), -1, dtype=torch.int32)
+        self.seq_pos = torch.zeros(self.max_seqs, dtype=torch.int32)
+        for i, s in enumerate(self.slots):
+            for j in range(need[i]):
+                self.table[s, j] = order.pop()
+            self.seq_pos[s] = pos[i]
+        self.start = [0]
+        for n in new:
+            self.start.append(self.start[-1] + n)
+        self.rows = self.start[-1] + spare_rows
+        self.codes = torch.randint(0, 256, (self.n_pages, layers, 2, nkv, PAGE, hd), dtype=torch.uint8, generator=g)
+        # every byte, NaN codes too, where nothing is cached; e4m3 values with larger ones rare where something is
+        x = (torch.randn(self.codes.shape, generator=g) * 60).clamp(-448, 448).to(torch.float8_e4m3fn)
+        x = x.view(torch.uint8)
+        for i, s in enumerate(self.slots):
+            for j in range(pos[i]):
+                p = int(self.table[s, j // PAGE])
+                self.codes[p, :, :, :, j % PAGE] = x[p, :, :, :, j % PAGE]
+        e = torch.randint(-9, -5, (self.n_pages, layers, 2, nkv, PAGE // 16), generator=g)
+        self.scales = torch.exp2(e.float()) * size
+        self.device()
+
+    def device(self):
+        d = lambda t: t.cuda()  # noqa: E731
+        self.d_codes, self.d_scales, self.d_table = d(self.codes), d(self.scales), d(self.table)
+        self.d_pos = d(self.seq_pos)
+        self.d_slots = d(torch.tensor([-1 if i in self.unused else s for i, s in enumerate(self.slots)],
+                                      dtype=torch.int32))
+        self.d_start = d(torch.tensor(self.start, dtype=torch.int32))
+        self.d_err = torch.zeros(1, dtype=torch.int32, device="cuda")
+        self.max_new = max(1, max(self.new))
+        self.max_ctx = max(1, max(p + n for p, n in zip(self.pos, self.new)))
+        self.cache = Kv8Cache(self.n_pages, self.layers, self.nkv, self.hd, self.max_seqs, self.max_pages,
+                              ptr(self.d_codes), ptr(self.d_scales), ptr(self.d_table), ptr(self.d_pos),
+                              ptr(self.d_err))
+        half = self.hd // 2
+        ang = torch.arange(self.max_ctx).double()[:, None] * 1e4 ** (-torch.arange(half).double() / half)
+        self.cos, self.sin = ang.cos().float(), ang.sin().float()
+        self.d_cos, self.d_sin = self.cos.cuda(), self.sin.cuda()
+
+    def use_start(self):
+        return None if self.rows == self.seqs and set(self.new) == {1} else ptr(self.d_start)
+
+    def status(self):
+        return lib().mmc_op_kv8_status(self.cache, None)
+
+    def append(self, qkv, qn=None, kn=None, q=None, stream=None, start="auto"):
+        q = torch.full((self.rows, self.nq * self.hd), 7.0, dtype=torch.float16, device="cuda") if q is None else q
+        check(lib().mmc_op_kv8_append(self.cache, self.layer, self.seqs, self.rows, self.max_new, ptr(self.d_slots),
+                                      self.use_start() if start == "auto" else start, self.nq, ptr(qkv), ptr(qn),
+                                      ptr(kn), ptr(self.d_cos), ptr(self.d_sin), self.max_ctx, EPS, ptr(q), stream))
+        return q
+
+    def workspace(self, max_ctx=None):
+        n = C.c_size_t()
+        check(lib().mmc_op_kv8_attention_workspace_size(self.cache, self.seqs, self.rows, self.max_new, self.nq,
+                                                        max_ctx or self.max_ctx, C.byref(n)))
+        return torch.full((n.value,), 0xff, dtype=torch.uint8, device="cuda")  # NaN as floats
+
+    def attend(self, q, out=None, ws=None, stream=None, max_ctx=None):
+        out = torch.full((self.rows, self.nq * self.hd), 7.0, dtype=torch.float16, device="cuda") if out is None else out
+        ws = self.workspace(max_ctx) if ws is None else ws
+        check(lib().mmc_op_kv8_attention(self.cache, self.layer, self.seqs, self.rows, self.max_new, ptr(self.d_slots),
+                                         self.use_start(), self.nq, ptr(q), max_ctx or self.max_ctx, ptr(out), ptr(ws),
+                                         ws.numel(), stream))
+        return out
+
+    # ---- checks against the 64-bit forms
+    def check_append(self, qkv, qn, kn, q):
+        nq, nkv, hd, lay = self.nq, self.nkv, self.hd, self.layer
+        ref = Cache(self.codes, self.scales)
+        got_c = e4m3_table()[self.d_codes.cpu().long()]
+        got_s = self.d_scales.cpu().double()
+        x = qkv.cpu().view(self.rows, nq + 2 * nkv, hd)
+        q = q.cpu().double().view(self.rows, nq, hd)
+        for i in range(self.seqs):
+            r0, r1, p0, n = self.start[i], self.start[i + 1], self.pos[i], self.new[i]
+            if i in self.unused:
+                assert (q[r0:r1] == 7).all()
+                continue
+            if n == 0:
+                continue
+            cos, sin = self.cos[p0:p0 + n, None], self.sin[p0:p0 + n, None]
+            want = norm_rope(x[r0:r1, :nq], qn, cos, sin, EPS)
+            # fp32: the norm's sum and factors and two products and a sum, each 2^-24 of the pair's size; fp16: half a step
+            a, b = norm_rope(x[r0:r1, :nq], qn, torch.ones_like(cos), torch.zeros_like(sin), EPS).abs().chunk(2, -1)
+            pair = torch.cat([a + b, a + b], -1)
+            assert ((q[r0:r1] - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -25 + (hd + 16) * 2.0 ** -24 * pair).all()
+            k = norm_rope(x[r0:r1, nq:nq + nkv], kn, cos, sin, EPS)
+            ref.append(lay, self.table[self.slots[i]], p0, torch.stack([k, x[r0:r1, nq + nkv:].double()]).transpose(1, 2))
+        live = ~got_s.isnan()
+        assert torch.equal(live, ~ref.scales.isnan())
+        assert torch.equal(got_s[live], ref.scales[live])
+        # V has no arithmetic before its code: equal. K may fall on the other side of a border where fp32 and 64 bits
+        # differ: by one step (an eighth of the value, 2^-9 at least), and seldom
+        same = (got_c == ref.codes) | (got_c.isnan() & ref.codes.isnan())
+        assert same[:, :, 1].all()
+        diff = ~same[:, :, 0]
+        assert diff.sum() <= max(2, 1e-3 * self.start[-1] * nkv * hd)
+        g, w = got_c[:, :, 0][diff], ref.codes[:, :, 0][diff]
+        assert ((g - w).abs() <= torch.maximum(w.abs(), g.abs()) / 8 + 2.0 ** -9).all()
+
+    def check_attention(self, q, out, rows=None):
+        ref = Cache(self.d_codes.cpu(), self.d_scales.cpu())
+        q, out = q.cpu(), out.cpu().double()
+        worst = 0.0
+        for i in range(self.seqs):
+            n = self.pos[i] + self.new[i]
+            if self.new[i] == 0:
+                continue
+            r0 = self.start[i]
+            if i in self.unused:
+                assert (out[r0:r0 + self.new[i]] == 0).all()
+                continue
+            kv = ref.read(self.layer, self.table[self.slots[i]], n)
+            for j in range(self.new[i]):
+                want, tol = attention(q[r0 + j].view(self.nq, self.hd), kv, self.pos[i] + j)
+                err = (out[r0 + j].view(self.nq, self.hd) - want).abs()
+                assert (err <= tol).all(), (i, j, float((err / tol).max()))
+                worst = max(worst, float((err / tol).max()))
+        assert (out[self.start[-1]:] == 7).all()  # rows behind the last sequence
+        return worst
+
+
+def qkv_of(w, size=1.0):
+    x = torch.randn(w.rows, (w.nq + 2 * w.nkv) * w.hd, generator=w.g) * size
+    return x.cuda()
+
+
+def q_of(w, size=1.5):
+    return (torch.randn(w.rows, w.nq * w.hd, generator=w.g) * size).half().cuda()
+
+
+def norms_of(w):
+    return [(1 + 0.2 * torch.randn(w.hd, generator=w.g)) for _ in range(2)]
+
+
+SHAPES = [(8, 2, 64), (8, 2, 96), (4, 4, 16), (6, 2, 32), (10, 2, 128), (7, 1, 96), (40, 2, 64), (3, 3, 128)]
+
+# positions before the call, new rows
+BATCHES = {
+    "one": ([0], [1]),
+    "steps": ([0, 1, 15, 16, 17, 63, 64, 65, 200, 511, 1000], [1] * 11),
+    "several": ([0, 3, 14, 60, 129, 300], [2, 5, 3, 8, 0, 7]),
+    "prompts": ([0, 5, 64, 0], [130, 75, 64, 1]),
+}
+
+
+@pytest.mark.parametrize("batch", BATCHES)
+@pytest.mark.parametrize("nq,nkv,hd", SHAPES)
+def test_append(nq, nkv, hd, batch):
+    pos, new = BATCHES[batch]
+    w = World(hd * 7 + nq, nq, nkv, hd, pos, new, layers=2, layer=1)
+    x = qkv_of(w)
+    qn, kn = norms_of(w) if nq != 7 else (None, None)
+    q = w.append(x, qn.cuda() if qn is not None else None, kn.cuda() if kn is not None else None)
+    assert w.status() == 0
+    w.check_append(x, qn, kn, q)
+
+
+@pytest.mark.parametrize("batch", BATCHES)
+@pytest.mark.parametrize("nq,nkv,hd", SHAPES)
+def test_attention(nq, nkv, hd, batch):
+    pos, new = BATCHES[batch]
+    w = World(hd * 9 + nq, nq, nkv, hd, pos, new, layers=2, layer=0)
+    # the new positions hold values too: append before attending
+    w.append(qkv_of(w))
+    q = q_of(w)
+    out = w.attend(q)
+    assert w.status() == 0
+    w.check_attention(q, out)
+
+
+@pytest.mark.parametrize("nq,nkv,hd,pos,new", [
+    (8, 2, 96, [8191], [1]), (8, 2, 64, [20000], [1]), (16, 8, 128, [5000, 0, 77], [1, 1, 1]),
+    (8, 2, 96, [4000, 1500], [5, 33]), (8, 1, 32, [32700], [4]), (64, 1, 64, [900], [3])])
+def test_attention_long(nq, nkv, hd, pos, new):
+    w = World(sum(pos) + hd, nq, nkv, hd, pos, new)
+    w.append(qkv_of(w))
+    q = q_of(w)
+    out = w.attend(q)
+    assert w.status() == 0
+    w.check_attention(q, out)
+
+
+def test_attention_many_sequences():
+    g = torch.Generator().manual_seed(11)
+    pos = torch.randint(0, 700, (256,), generator=g).tolist()
+    w = World(12, 8, 2, 96, pos, [1] * 256)
+    w.append(qkv_of(w))
+    q = q_of(w)
+    out = w.attend(q)
+    assert w.status() == 0
+    w.check_attention(q, out)
+
+
+def test_unused_rows_and_spare_rows():
+    """A padded batch: unused sequences, rows behind the last one."""
+    w = World(5, 8, 2, 64, [70, 10, 33, 5], [3, 2, 1, 4], spare_rows=5, unused=(1, 3))
+    before = w.d_codes.clone(), w.d_scales.clone()
+    x = qkv_of(w)
+    q = w.append(x)
+    assert w.status() == 0
+    assert (q[w.start[-1]:] == 7).all()
+    w.check_append(x, None, None, q)
+    for i in (1, 3):
+        pages = [p for p in w.table[w.slots[i]].tolist() if p >= 0]
+        assert torch.equal(w.d_codes[pages], before[0][pages]) and torch.equal(w.d_scales[pages], before[1][pages])
+    qq = q_of(w)
+    out = w.attend(qq)
+    assert w.status() == 0
+    w.check_attention(qq, out)
+
+
+def test_nothing_to_do():
+    """Every sequence unused, or without rows."""
+    w = World(6, 8, 2, 64, [70, 10], [1, 1], unused=(0, 1))
+    out = w.attend(q_of(w))
+    assert w.status() == 0 and (out == 0).all()
+    w = World(7, 8, 2, 64, [70, 10], [0, 0], spare_rows=3)
+    before = w.d_codes.clone()
+    q = w.append(qkv_of(w))
+    out = w.attend(q_of(w))
+    assert w.status() == 0 and (out == 7).all() and (q == 7).all() and torch.equal(w.d_codes, before)
+
+
+@pytest.mark.parametrize("hd", [16, 64, 96, 128])
+def test_growing_scales_step_by_step(hd):
+    """Tokens of growing, shrinking, zero and huge sizes, one a call: each step equals the 64-bit form applied to the
+    cache that the step found, and the V codes equal those of one append of all of them (scales are powers of two; the
+    sizes here keep every older code normal)."""
+    n = 40
+    size = [0.0, 1.0, 1.9, 0.5, 3.0, 8.0, 7.0, 20.0] * 5
+    w = World(hd, 4, 2, hd, [0], [n])
+    base = torch.randn(n, (w.nq + 2 * w.nkv) * hd, generator=w.g).sign() * (
+        0.75 + 0.25 * torch.rand(n, (w.nq + 2 * w.nkv) * hd, generator=w.g))
+    x = (base * torch.tensor(size)[:, None]).cuda()
+    w.append(x)
+    whole = w.d_codes.clone(), w.d_scales.clone()
+    one = World(hd, 4, 2, hd, [0], [n])
+    one.rows, one.max_new, one.new, one.start = 1, 1, [1], [0, 1]
+    for i in range(n):
+        one.codes, one.scales = one.d_codes.cpu(), one.d_scales.cpu()
+        one.pos = [i]
+        one.d_pos[one.slots[0]] = i
+        row = x[i:i + 1].contiguous()
+        q = one.append(row)
+        assert one.status() == 0
+        one.check_append(row, None, None, q)
+    used = [int(p) for p in w.table[w.slots[0]] if p >= 0]
+    t = e4m3_table()
+    for tok in range(n):
+        p, r = used[tok // PAGE], tok % PAGE
+        a, b = t[whole[0][p, 0, 1, :, r].cpu().long()], t[one.d_codes[p, 0, 1, :, r].cpu().long()]
+        assert torch.equal(a, b)
+    assert torch.equal(whole[1][used][:, 0, 1, :, :2], one.d_scales[used][:, 0, 1, :, :2])
+
+
+@pytest.mark.parametrize("amax", [448.0, 448.00003, 449.0, 3.4e38, 1.75 * 2.0 ** -126, 1e-40, 1e-45, 0.0])
+def test_scale_borders(amax):
+    w = World(3, 2, 2, 32, [3, 16], [2, 1])
+    x = qkv_of(w, 0.1 * min(amax, 1e37))
+    x[:, -w.nkv * w.hd:].clamp_(-amax, amax)
+    x[0, -1] = amax
+    x[2, -w.hd - 5] = -amax
+    q = w.append(x)
+    assert w.status() == 0
+    if 1e-38 < amax < 1e37:  # (q and K pass through products that leave fp32's range elsewhere)
+        w.check_append(x, None, None, q)
+        return
+    ref = Cache(w.codes, w.scales)
+    v = x.cpu().view(w.rows, w.nq + 2 * w.nkv, w.hd)[:, -w.nkv:].double()
+    for i in range(w.seqs):
+        vi = v[w.start[i]:w.start[i + 1]].transpose(0, 1)
+        ref.append(0, w.table[w.slots[i]], w.pos[i], torch.stack([vi, vi]))
+    assert torch.equal(w.d_scales.cpu().double()[:, :, 1], ref.scales[:, :, 1])
+    got = e4m3_table()[w.d_codes.cpu().long()][:, :, 1]
+    assert ((got == ref.codes[:, :, 1]) | got.isnan()).all()
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_infinite_values(bad):
+    """A block with an infinity or a NaN has the scale NaN from then on; every row that reads it is NaN, no other."""
+    w = World(8, 8, 2, 64, [20, 20], [2, 2])
+    x = qkv_of(w)
+    x[1, -3] = bad  # V of the last kv head, second row of sequence 0
+    q = w.append(x)
+    assert w.status() == 0
+    w.check_append(x, None, None, q)
+    qq = q_of(w)
+    out = w.attend(qq).cpu().view(4, 2, -1)
+    assert out[:2, 1].isnan().all() and not out[:2, 0].isnan().any() and not out[2:].isnan().any()
+    # later positions of that block: its scale stays NaN, its older codes stay
+    w2 = World(8, 8, 2, 64, [22, 22], [2, 2])
+    w2.d_codes.copy_(w.d_codes)
+    w2.d_scales.copy_(w.d_scales)
+    w2.codes, w2.scales = w.d_codes.cpu(), w.d_scales.cpu()
+    x = qkv_of(w2)
+    q = w2.append(x)
+    assert w2.status() == 0
+    w2.check_append(x, None, None, q)
+    assert w2.d_scales.isnan().sum() == 1
+
+
+def test_attention_extreme_scores():
+    """Scores of thousands, equal scores, rows whose largest score comes last, blocks of very different V sizes."""
+    for size, qs in ((1.0, 60000.0), (1.0, 0.0), (2.0 ** -20, 300.0), (2.0 ** 20, 3.0)):
+        w = World(21, 8, 2, 96, [700, 64], [1, 2], size=size)
+        w.d_scales[:, :, 1] *= torch.exp2(torch.randint(-20, 20, w.d_scales[:, :, 1].shape, generator=w.g).float()).cuda()
+        w.append(qkv_of(w, size))
+        q = (torch.randn(w.rows, w.nq * w.hd, generator=w.g).clamp(-1, 1) * qs).half().cuda()
+        out = w.attend(q)
+        assert w.status() == 0
+        ref = Cache(w.d_codes.cpu(), w.d_scales.cpu())
+        for i in range(w.seqs):
+            kv = ref.read(0, w.table[w.slots[i]], w.pos[i] + w.new[i])
+            for j in range(w.new[i]):
+                r = w.start[i] + j
+                want, tol = attention(q[r].cpu().view(w.nq, w.hd), kv, w.pos[i] + j)
+                got = out[r].cpu().double().view(w.nq, w.hd)
+                top = want.abs() + tol >= 65519  # past fp16: infinite or the largest value
+                assert ((got - want).abs()[~top] <= tol[~top]).all()
+
+
+def test_bad_pages_slots_and_rows_are_reported():
+    """Device-side refusals: each is reported once, then the word is clear; nothing outside is touched."""
+    def fresh():
+        return World(31, 8, 2, 64, [100, 40], [2, 3])
+
+    w = fresh()
+    w.d_table[w.slots[0], 1] = w.n_pages  # the page of positions 64..127
+    before = w.d_codes.clone()
+    w.append(qkv_of(w))
+    assert w.status() == DEVICE_ERROR and b"page" in lib().mmc_last_error() and w.status() == 0
+    w.attend(q_of(w))
+    assert w.status() == DEVICE_ERROR and b"page" in lib().mmc_last_error() and w.status() == 0
+    other = [p for p in w.table[w.slots[1]].tolist() if p >= 0]
+    rest = [p for p in range(w.n_pages) if p not in other]
+    assert torch.equal(w.d_codes[rest], before[rest])
+
+    w = fresh()
+    w.d_slots[0] = w.max_seqs
+    q = w.append(qkv_of(w))
+    assert w.status() == DEVICE_ERROR and b"slot" in lib().mmc_last_error()
+    out = w.attend(q_of(w))
+    assert w.status() == DEVICE_ERROR and (out[:2] == 7).all() and (q[:2] == 7).all() and not (out[2:] == 7).any()
+
+    w = fresh()
+    w.d_slots[0] = w.d_slots[1]
+    before = w.d_codes.clone()
+    w.append(qkv_of(w))
+    assert w.status() == DEVICE_ERROR and b"same slot" in lib().mmc_last_error()
+    assert torch.equal(w.d_codes, before)
+
+    for pos in (-1, w.max_pages * PAGE - 1, 2 ** 31 - 1):
+        w = fresh()
+        w.d_pos[w.slots[0]] = pos
+        before = w.d_codes.clone()
+        w.append(qkv_of(w))
+        assert w.status() == DEVICE_ERROR
+        out = w.attend(q_of(w))
+        assert w.status() == DEVICE_ERROR and (out[:2] == 7).all()
+
+    for start in ([0, 2, 6], [0, -2, 3], [-1, 2, 5], [0, 5, 5], [0, 2, 2 ** 31 - 1]):
+        w = fresh()
+        w.d_start.copy_(torch.tensor(start, dtype=torch.int32))
+        w.append(qkv_of(w))
+        w.status()
+        w.attend(q_of(w))
+        assert w.status() == DEVICE_ERROR
+
+    w = fresh()
+    w.max_ctx -= 1
+    w.attend(q_of(w), max_ctx=w.max_ctx)
+    assert w.status() == DEVICE_ERROR and b"max_ctx" in lib().mmc_last_error()
+
+
+def test_small_workspace_and_host_memory_are_refused():
+    w = World(1, 8, 2, 64, [3000], [1])
+    q, n = q_of(w), w.workspace().numel()
+    if n > 16:
+        out = torch.empty_like(q)
+        assert lib().mmc_op_kv8_attention(w.cache, 0, 1, 1, 1, ptr(w.d_slots), None, 8, ptr(q), w.max_ctx, ptr(out),
+                                          ptr(out), n - 1, None) == 1
+    host = torch.zeros(1 << 12)
+    aligned = (host.data_ptr() + 63) // 64 * 64
+    assert lib().mmc_op_kv8_attention(w.cache, 0, 1, 1, 1, ptr(w.d_slots), None, 8, aligned, w.max_ctx, ptr(q), ptr(q),
+                                      1 << 30, None) == 1
+    assert lib().mmc_op_w4_projection(1, 16, 64, 64, aligned, ptr(q), None, ptr(q), ptr(q), None) == 1
+
+
+# ------------------------------------------------------------------ 4-bit projections
+
+def w4_case(n, k, batch, group, zeros, seed=0, big=False):
+    g = torch.Generator().manual_seed(n * 3 + k + batch + seed)
+    codes = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, generator=g)
+    scales = (0.01 * torch.exp(torch.randn(n, k // group, generator=g))).half()
+    z = torch.randint(0, 256 if big else 16, (n, k // group), dtype=torch.uint8, generator=g) if zeros else None
+    x = (torch.randn(batch, k, generator=g) * torch.exp(torch.randn(k, generator=g))).half()
+    return codes, scales, z, x
+
+
+def w4_run(codes, scales, z, x, group, stream=None, y=None):
+    d = [t.cuda() if t is not None else None for t in (codes, scales, z, x)]
+    n, b, k = codes.shape[0], x.shape[0], x.shape[1]
+    y = torch.full((b + 1, n), 7.0, device="cuda") if y is None else y
+    check(lib().mmc_op_w4_projection(b, n, k, group, *(ptr(t) for t in d), ptr(y), stream))
+    torch.cuda.synchronize()
+    assert (y[b:] == 7).all()
+    return y[:b].cpu().double()
+
+
+def w4_check(codes, scales, z, x, group):
+    y = w4_run(codes, scales, z, x, group)
+    w = w4_weights(codes, scales, z, group)
+    want = x.double() @ w.T
+    # products are exact; every value passes at most group / 16 sums of a group, k / group sums over groups and 16 joins,
+    # each off by 2^-23 (truncating adders) of what it holds at most: sum |w x|
+    k = x.shape[1]
+    tol = (group // 16 + 16 + k // group + 32) * 2.0 ** -23 * (x.double().abs() @ w.abs().T) + 1e-30
+    assert ((y - want).abs() <= tol).all(), float(((y - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("n,k", [(768, 768), (1152, 768), (17, 128), (1, 128), (2048, 768), (100, 2432), (515, 1408)])
+@pytest.mark.parametrize("batch", [1, 3, 8, 9, 24, 64])
+def test_w4_projection(n, k, batch, group, zeros):
+    if k % group:
+        pytest.skip("group does not divide k")
+    w4_check(*w4_case(n, k, batch, group, zeros, big=n == 17), group)
+
+
+@pytest.mark.parametrize("n,k,batch,group,zeros", [(16, 32, 1, 32, True), (5, 96, 2, 32, False), (33, 160, 7, 32, True),
+                                                   (300, 16384, 1, 128, False), (64, 8192, 17, 64, True),
+                                                   (40, 768, 130, 32, True), (4096, 4096, 33, 128, False),
+                                                   (6400, 768, 65, 64, True), (20000, 256, 5, 32, False)])
+def test_w4_projection_sizes(n, k, batch, group, zeros):
+    w4_check(*w4_case(n, k, batch, group, zeros), group)
+
+
+def test_w4_projection_repeats_and_special_values():
+    """Equal runs give equal bits; an infinite scale or input shows only in its own outputs."""
+    codes, scales, z, x = w4_case(200, 512, 5, 64, True)
+    a = w4_run(codes, scales, z, x, 64)
+    for _ in range(3):
+        assert torch.equal(a, w4_run(codes, scales, z, x, 64))
+    scales[7, 3] = math.nan
+    x[2, 100] = math.inf
+    b = w4_run(codes, scales, z, x, 64)
+    assert b[:, 7].isnan().all() and not torch.isfinite(b[2]).any()
+    keep = torch.ones_like(a, dtype=torch.bool)
+    keep[:, 7] = False
+    keep[2] = False
+    assert torch.equal(a[keep], b[keep])
+
+
+# ------------------------------------------------------------------ a run of them together
+
+def test_quantised_block_runs_together():
+    """The attention block of a small model with 4-bit weights and the 8-bit cache: a prompt pass and single steps of
+    ragged sequences. Each operator's output is checked against its 64-bit form on the inputs it found; the steps are
+    then repeated from the same state as one captured graph, on another stream, with equal bits."""
+    hidden, nq, nkv, hd, group = 256, 8, 2, 64, 64
+    qdim, odim = (nq + 2 * nkv) * hd, nq * hd
+    pos, new = [0, 0, 0], [37, 5, 64]
+    w = World(77, nq, nkv, hd, [80, 80, 80], [1, 1, 1])  # pages for 80 positions and more
+    qn, kn = [t.cuda() for t in norms_of(w)]
+    W = {}
+    for name, n, k in (("qkv", qdim, hidden), ("o", hidden, odim)):
+        c, s, z, _ = w4_case(n, k, 1, group, True)
+        W[name] = (c, s * 0.3, z, [t.cuda() for t in (c, s * 0.3, z)])
+
+    def project(name, x, y, stream=None):
+        c, s, z, d = W[name]
+        check(lib().mmc_op_w4_projection(x.shape[0], c.shape[0], x.shape[1], group, *(ptr(t) for t in d), ptr(x), ptr(y),
+                                         stream))
+
+    def check_project(name, x, y):
+        c, s, z, _ = W[name]
+        wt = w4_weights(c, s, z, group)
+        xs = x.cpu().double()
+        tol = (group // 16 + 16 + x.shape[1] // group + 32) * 2.0 ** -23 * (xs.abs() @ wt.abs().T) + 1e-30
+        assert ((y.cpu().double() - xs @ wt.T).abs() <= tol).all()
+
+    def step(x, checked):
+        """x [rows][hidden] fp16 -> the block's output, every stage checked."""
+        y = torch.empty(w.rows, qdim, device="cuda")
+        o = torch.empty(w.rows, hidden, device="cuda")
+        project("qkv", x, y)
+        w.codes, w.scales = w.d_codes.cpu(), w.d_scales.cpu()
+        q = w.append(y, qn, kn)
+        att = w.attend(q)
+        project("o", att, o)
+        assert w.status() == 0
+        if checked:
+            check_project("qkv", x, y)
+            w.check_append(y, qn.cpu(), kn.cpu(), q)
+            w.check_attention(q, att)
+            check_project("o", att, o)
+        return o
+
+    def batch(pos, new):
+        w.pos, w.new = list(pos), list(new)
+        w.start = [0]
+        for n in new:
+            w.start.append(w.start[-1] + n)
+        w.rows, w.max_new = w.start[-1], max(new)
+        w.d_start.copy_(torch.tensor(w.start, dtype=torch.int32))
+        for i, s in enumerate(w.slots):
+            w.d_pos[s] = pos[i]
+
+    batch(pos, new)
+    x = torch.randn(w.rows, hidden, generator=w.g).half().cuda()
+    step(x, True)
+    pos = [p + n for p, n in zip(pos, new)]
+    saved, steps = None, []
+    for i in range(6):
+        batch(pos, [1, 1, 1])
+        if i == 0:
+            saved = w.d_codes.clone(), w.d_scales.clone(), w.d_pos.clone()
+        x = torch.randn(3, hidden, generator=w.g).half().cuda()
+        steps.append((x, step(x, True)))
+        pos = [p + 1 for p in pos]
+    # the same steps as replays of one graph
+    w.d_codes.copy_(saved[0])
+    w.d_scales.copy_(saved[1])
+    w.d_pos.copy_(saved[2])
+    xs = torch.empty(3, hidden, dtype=torch.float16, device="cuda")
+    y = torch.empty(3, qdim, device="cuda")
+    q, att = (torch.empty(3, odim, dtype=torch.float16, device="cuda") for _ in range(2))
+    o = torch.empty(3, hidden, device="cuda")
+    ws = w.workspace()
+    idx = torch.tensor(w.slots, device="cuda")
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        s = torch.cuda.current_stream().cuda_stream
+        project("qkv", xs, y, s)
+        w.append(y, qn, kn, q, s)
+        w.attend(q, att, ws, s)
+        project("o", att, o, s)
+        w.d_pos[idx] += 1
+    torch.cuda.synchronize()
+    for x, want in steps:
+        xs.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want)
+    assert w.status() == 0
+
+
+def test_two_streams_with_a_workspace_each():
+    """Calls side by side on two streams, each with its own workspace and outputs, equal the calls alone."""
+    ws = [World(s, 8, 2, 96, [1500 + s, 300], [1, 1]) for s in (1, 2)]
+    qs = [q_of(w) for w in ws]
+    for w in ws:
+        w.append(qkv_of(w))
+    alone = [w.attend(q) for w, q in zip(ws, qs)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in ws]
+    space = [w.workspace() for w in ws]
+    outs = [torch.full_like(a, 7.0) for a in alone]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for w, q, s, sp, o in zip(ws, qs, streams, space, outs):
+            w.attend(q, o, sp, s.cuda_stream)
+    torch.cuda.synchronize()
+    for a, o in zip(alone, outs):
+        assert torch.equal(a, o)
