@@ -49,12 +49,15 @@ struct Kv8AttnArgs {
   const __half* q = nullptr;  // [rows][nq * hd]
   __half* out = nullptr;      // [rows][nq * hd]
   int max_ctx = 0;
-  int splits = 1;         // parts of each sequence's pages
-  float* part = nullptr;  // splits > 1: kv8_part_floats(...)
+  int split_pages = 1, splits = 1;  // pages of a part, parts of max_ctx positions
+  float* part = nullptr;            // splits > 1: the plan's part_floats
 };
-// splits of a call over `sms` SMs
-int kv8_plan_splits(int n_seqs, int max_new, int nq, int nkv, int max_ctx, int sms);
-size_t kv8_part_floats(int n_seqs, int max_new, int nq, int nkv, int hd, int splits);
+// How a call is split over `sms` SMs.
+struct Kv8Plan {
+  int split_pages = 1, splits = 1;
+  size_t part_floats = 0;
+};
+Kv8Plan kv8_plan(int n_seqs, int max_new, int nq, int nkv, int hd, int max_ctx, int sms);
 cudaError_t launch_kv8_attention(const Kv8AttnArgs& a, int hd, cudaStream_t s);
 cudaError_t kv8_init_attributes();
 

@@ -174,8 +174,8 @@ int mmc_op_kv8_attention_workspace_size(const mmc_kv8_cache* cache, int32_t n_se
     check_batch(cache, n_seqs, rows, max_new, nq);
     require(bytes != nullptr, "null argument");
     require(max_ctx >= 1, "max_ctx must be at least 1");
-    const int splits = mmc::kv8_plan_splits(n_seqs, max_new, nq, cache->nkv, max_ctx, prepare_device());
-    *bytes = std::max<size_t>(16, mmc::kv8_part_floats(n_seqs, max_new, nq, cache->nkv, cache->hd, splits) * 4);
+    const mmc::Kv8Plan p = mmc::kv8_plan(n_seqs, max_new, nq, cache->nkv, cache->hd, max_ctx, prepare_device());
+    *bytes = std::max<size_t>(16, p.part_floats * 4);
   });
 }
 
@@ -193,9 +193,10 @@ int mmc_op_kv8_attention(const mmc_kv8_cache* cache, int32_t layer, int32_t n_se
     on_device(cache->d_codes, "d_codes is not memory of the current device");
     on_device(d_q_fp16, "d_q is not memory of the current device");
     on_device(d_out_fp16, "d_out is not memory of the current device");
-    a.splits = mmc::kv8_plan_splits(n_seqs, max_new, nq, cache->nkv, max_ctx, prepare_device());
-    require(workspace_bytes >= mmc::kv8_part_floats(n_seqs, max_new, nq, cache->nkv, cache->hd, a.splits) * 4,
-            "workspace too small");
+    const mmc::Kv8Plan p = mmc::kv8_plan(n_seqs, max_new, nq, cache->nkv, cache->hd, max_ctx, prepare_device());
+    require(workspace_bytes >= std::max<size_t>(16, p.part_floats * 4), "workspace too small");
+    a.split_pages = p.split_pages;
+    a.splits = p.splits;
     a.q = static_cast<const __half*>(d_q_fp16);
     a.out = static_cast<__half*>(d_out_fp16);
     a.max_ctx = max_ctx;

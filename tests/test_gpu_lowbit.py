@@ -339,6 +339,25 @@ def test_infinite_values(bad):
     assert w2.d_scales.isnan().sum() == 1
 
 
+def test_infinite_value_ahead_of_a_row():
+    """Rows that see no position of a lost block are not touched by it, though they share its tile."""
+    for pos in (14, 62, 0):
+        w = World(9, 8, 2, 96, [pos], [18])
+        x = qkv_of(w)
+        x[17, :] = math.nan  # q, K and V of the last row
+        w.append(x)
+        q = q_of(w)
+        out = w.attend(q)
+        assert w.status() == 0
+        free = (pos + 17) // 16 * 16 - pos  # rows before the lost block
+        ref = Cache(w.d_codes.cpu(), w.d_scales.cpu())
+        kv = ref.read(0, w.table[w.slots[0]], pos + free) if free else None
+        for j in range(free):
+            want, tol = attention(q[j].cpu().view(w.nq, w.hd), kv, pos + j)
+            assert ((out[j].cpu().double().view(w.nq, w.hd) - want).abs() <= tol).all()
+        assert out[free:].isnan().all()
+
+
 def test_attention_extreme_scores():
     """Scores of thousands, equal scores, rows whose largest score comes last, blocks of very different V sizes."""
     for size, qs in ((1.0, 60000.0), (1.0, 0.0), (2.0 ** -20, 300.0), (2.0 ** 20, 3.0)):
