@@ -91,6 +91,7 @@ void check_batch(const mmc_kv8_cache* c, int32_t n_seqs, int32_t rows, int32_t m
   require(n_seqs >= 1 && n_seqs <= 65535, "n_seqs must be in 1..65535");
   require(rows >= 1 && max_new >= 1 && max_new <= rows, "rows and max_new must be at least 1, max_new at most rows");
   require((int64_t)max_new * (nq / c->nkv) <= (int64_t(1) << 24), "max_new * (nq / nkv) is too large");
+  require((int64_t)c->n_pages * c->layers * 2 * c->nkv < (int64_t(1) << 31), "n_pages * layers * 2 * nkv is too large");
 }
 
 mmc::Kv8Args make_args(const mmc_kv8_cache* c, int32_t layer, int32_t n_seqs, int32_t rows, int32_t max_new,
@@ -100,7 +101,7 @@ mmc::Kv8Args make_args(const mmc_kv8_cache* c, int32_t layer, int32_t n_seqs, in
           "null cache, slots or error pointer");
   require(row_start != nullptr || (rows == n_seqs && max_new == 1),
           "without d_row_start each sequence has one row: rows == n_seqs, max_new == 1");
-  require(aligned(c->d_codes, 16), "d_codes must be 16-byte aligned");
+  require(aligned(c->d_codes, 16) && aligned(c->d_scales, 16), "d_codes and d_scales must be 16-byte aligned");
   mmc::Kv8Args k;
   k.codes = static_cast<uint8_t*>(c->d_codes);
   k.scales = c->d_scales;

@@ -40,7 +40,7 @@ BATCHES = [dict(layer=2), dict(layer=-1), dict(n_seqs=0), dict(n_seqs=65536, row
            dict(nq=3), dict(nq=0), dict(nq=-2)]
 CACHES = [dict(hd=48), dict(hd=0), dict(hd=256), dict(n_pages=0), dict(layers=0), dict(nkv=0), dict(max_seqs=0),
           dict(max_pages=0), dict(d_codes=None), dict(d_scales=None), dict(d_block_table=None), dict(d_seq_pos=None),
-          dict(d_error=None), dict(d_codes=P + 8)]
+          dict(d_error=None), dict(d_codes=P + 8), dict(d_scales=P + 4), dict(n_pages=1 << 30)]
 
 
 @pytest.mark.parametrize("kw", BATCHES + [dict(qkv=None), dict(qn=None), dict(kn=None), dict(cos=None),
