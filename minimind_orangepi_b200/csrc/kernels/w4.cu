@@ -1,7 +1,7 @@
 // Projections with weights in 4 bits: y[b][n] = sum_k (c[n][k] - z[n][k / G]) s[n][k / G] x[b][k].
 //
 // A CTA takes BM weight rows and 8 NT batch rows. Tensor copies stream the codes
-// and x through a ring; eight warps (WM down the rows, WK along the columns, 128
+// and x through a ring; the warps (WM down the rows, WK along the columns, 128
 // columns of each stage a warp) take them from there: codes by ldmatrix, less
 // their zero point in fp16 (exact), m16n8k16 with the weight rows on M, each
 // group's sum in fp32, then scaled. The warps' and, where a cluster shares the
@@ -16,19 +16,19 @@
 namespace mmc {
 namespace {
 
-constexpr int kW4Warps = 8;
-constexpr int kW4Threads = kW4Warps * 32;
 constexpr int kW4Part = 128;                     // columns of a stage that one warp takes
 
 template <int NT>
 struct W4Cfg {
+  static constexpr int WARPS = NT == 1 || NT == 8 ? 8 : 16, THREADS = WARPS * 32;
   static constexpr int MT = 2;                                   // 16-row tiles of a warp
-  static constexpr int WM = NT == 1 ? 1 : NT == 2 ? 2 : 4;       // warps down the rows
-  static constexpr int WK = kW4Warps / WM;                       // warps along the columns
+  static constexpr int WM = NT == 1 ? 1 : 4;                     // warps down the rows
+  static constexpr int WK = WARPS / WM;                          // warps along the columns
   static constexpr int BM = 16 * MT * WM, KC = kW4Part * WK;     // rows of a CTA, columns of a stage
-  static constexpr int W_BYTES = BM * KC / 2, X_BYTES = 8 * NT * KC * 2, STAGE = W_BYTES + X_BYTES;
-  static constexpr int STAGES = NT <= 2 ? 3 : 4;
-  static constexpr int CTAS = NT <= 2 ? 2 : 1;                   // of an SM
+  // up to eight batch rows are read by the lanes that need them; more go through the ring
+  static constexpr int W_BYTES = BM * KC / 2, X_BYTES = NT == 1 ? 0 : 8 * NT * KC * 2, STAGE = W_BYTES + X_BYTES;
+  static constexpr int CTAS = NT == 1 ? 2 : 1;                   // of an SM
+  static constexpr int STAGES = 208 * 1024 / CTAS / STAGE;
   static constexpr int JOIN = (WK + 1) * BM * 8 * NT * 4;
   static constexpr int RING = STAGE * STAGES > JOIN ? STAGE * STAGES : JOIN;
   static constexpr int SMEM = 1024 + RING + 2 * STAGES * 8;
@@ -46,13 +46,18 @@ __device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
 // Eight codes of one word less z, as pairs of columns (0, 4), (1, 5), (2, 6),
 // (3, 7). A code in the low mantissa bits of 1024 is 1024 + c, four bits up
 // 1024 + 16 c: exact, and so are the differences. z1024: 1024 + z, z64: -(64 + z).
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {  // (a & mask) | bits, one instruction
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(a), "r"(mask), "r"(bits));
+  return d;
+}
 __device__ __forceinline__ void codes_less(uint32_t w, uint32_t z1024, uint32_t z64, uint32_t (&h)[4]) {
   constexpr uint32_t sixteenth = 0x2c002c00u, low = 0x000f000fu, high = 0x00f000f0u, k1024 = 0x64006400u;
-  h[0] = h2_sub((w & low) | k1024, z1024);
-  h[1] = h2_fma((w & high) | k1024, sixteenth, z64);
+  h[0] = h2_sub(and_or(w, low, k1024), z1024);
+  h[1] = h2_fma(and_or(w, high, k1024), sixteenth, z64);
   w >>= 8;
-  h[2] = h2_sub((w & low) | k1024, z1024);
-  h[3] = h2_fma((w & high) | k1024, sixteenth, z64);
+  h[2] = h2_sub(and_or(w, low, k1024), z1024);
+  h[3] = h2_fma(and_or(w, high, k1024), sixteenth, z64);
 }
 __device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
@@ -65,12 +70,13 @@ __device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, in
 // and the call's outputs become NaN (there is no error word to set).
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, nullptr); }
 
-template <int NT, int GROUP>
-__global__ void __launch_bounds__(kW4Threads, W4Cfg<NT>::CTAS)
+template <int NT, int GROUP, bool ZEROS>
+__global__ void __launch_bounds__(W4Cfg<NT>::THREADS, W4Cfg<NT>::CTAS)
     w4_projection_kernel(const W4Args a, int parts, const __grid_constant__ CUtensorMap wmap,
                          const __grid_constant__ CUtensorMap xmap) {
   using C = W4Cfg<NT>;
-  constexpr int MT = C::MT, GP = kW4Part / GROUP;  // groups of a warp's columns in a stage
+  constexpr int MT = C::MT, CHUNKS = kW4Part / 32;
+  constexpr int CG = GROUP / 32, GP = kW4Part / GROUP;  // 32-column chunks of a group, groups of a warp's part
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::RING);
@@ -80,16 +86,13 @@ __global__ void __launch_bounds__(kW4Threads, W4Cfg<NT>::CTAS)
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   const int n0 = blockIdx.x / parts * C::BM, b0 = blockIdx.y * 8 * NT;
   const int all = (a.K + C::KC - 1) / C::KC, per = (all + parts - 1) / parts;
-  const int s0 = min(all, int(rank) * per), s1 = min(all, s0 + per);  // this CTA's stages of columns
+  const int s0 = min(all, int(rank) * per), n_st = min(all, s0 + per) - s0;  // this CTA's stages of columns
   if (tid < C::STAGES) {
     mbar_init(full + tid, 1);
-    mbar_init(empty + tid, kW4Warps);
+    mbar_init(empty + tid, C::WARPS);
   }
   fence_mbar_init();
   __syncthreads();
-  bool ok = true;
-  float acc[MT][NT][4] = {};
-  const int wm = warp % C::WM, wk = warp / C::WM;
   // thread 0 starts the copies of this CTA's i-th stage
   auto fill = [&](int i) {
     const int s = s0 + i, st = i % C::STAGES;
@@ -97,109 +100,145 @@ __global__ void __launch_bounds__(kW4Threads, W4Cfg<NT>::CTAS)
     mbar_arrive_expect_tx(full + st, C::STAGE);
 #pragma unroll
     for (int j = 0; j < C::KC / 256; ++j) load_2d(dst + j * C::BM * 128, &wmap, s * (C::KC / 2) + j * 128, n0, full + st);
+    if constexpr (NT > 1) {
 #pragma unroll
-    for (int j = 0; j < C::KC / 64; ++j)
-      load_2d(dst + C::W_BYTES + j * 8 * NT * 128, &xmap, s * C::KC + j * 64, b0, full + st);
+      for (int j = 0; j < C::KC / 64; ++j)
+        load_2d(dst + C::W_BYTES + j * 8 * NT * 128, &xmap, s * C::KC + j * 64, b0, full + st);
+    }
   };
-  int filled = min(C::STAGES, s1 - s0);
+  int filled = min(C::STAGES, n_st);
   if (tid == 0)
     for (int i = 0; i < filled; ++i) fill(i);
-  {
-    const int groups = a.K / GROUP;
-    // this lane's rows, n0 + wm * 32 + g + 8 r, and (of a stage's GP groups of this warp) group t
-    const int row0 = n0 + wm * 16 * MT + g;
-    auto fetch = [&](int s, uint32_t (&sc)[2 * MT], uint32_t (&z)[2 * MT]) {
-      const int gr = s * (C::KC / GROUP) + wk * GP + (t % GP);
-      const bool in = s < s1 && gr < groups;
+
+  const int wm = warp % C::WM, wk = warp / C::WM;
+  // this lane's weight rows n0 + 32 wm + g + 8 r; of a stage's GP groups of this warp it fetches the (t % GP)-th, a stage
+  // ahead. (Rows behind N repeat the last one and are not stored; groups behind K have x = 0 and the scale 0.)
+  const int groups = a.K / GROUP;
+  uint32_t at[2 * MT];
 #pragma unroll
-      for (int r = 0; r < 2 * MT; ++r) {
-        const bool here = in && row0 + 8 * r < a.N;
-        const size_t at = (size_t)(row0 + 8 * r) * groups + gr;
-        sc[r] = here ? __half_as_ushort(a.scales[at]) : 0u;
-        z[r] = here && a.zeros ? a.zeros[at] : 8u;
-      }
-    };
-    uint32_t sc[2 * MT], z[2 * MT];
-    fetch(s0, sc, z);
-    // ldmatrix: row `lane` of the warp's 32, 16-byte chunk 4 (wk & 1) + c of its 128-byte row
-    const uint32_t w_at = (wk >> 1) * C::BM * 128 + (wm * 32 + lane) * 128;
-    // x: batch row 8 nt + xr is column g of the n-tile, so that the eight lanes of a 16-byte read's phase fall on all banks
-    // of the swizzled rows
-    const int xr = (g & 1) * 4 + (g >> 1);
-    const uint32_t x_at = C::W_BYTES + wk * 2 * (8 * NT * 128) + xr * 128 + ((t ^ (xr & 3)) << 4);
-    for (int s = s0; s < s1; ++s) {
-      const int i = s - s0, st = i % C::STAGES;
-      uint32_t sc1[2 * MT], z1[2 * MT];
-      fetch(s + 1, sc1, z1);
-      ok = __all_sync(0xffffffffu, ok && wait(full + st, (i / C::STAGES) & 1));
-      if (!ok) break;
-      if (tid == 0 && i > 0 && i - 1 + C::STAGES < s1 - s0) {  // the stage before this one, once all warps have left it
-        ok = wait(empty + (i - 1) % C::STAGES, ((i - 1) / C::STAGES) & 1);
-        if (ok) fill(filled++);
-      }
-      const uint8_t* base = smem + st * C::STAGE;
-      const uint32_t base_u = smem_u32(base);
-      float d[MT][NT][4];
+  for (int r = 0; r < 2 * MT; ++r) at[r] = min(n0 + wm * 32 + g + 8 * r, a.N - 1) * uint32_t(groups);
+  int gr = s0 * (C::KC / GROUP) + wk * GP + t % GP;
+  uint32_t sc[2 * MT], z[2 * MT];
+  auto fetch_scale = [&](int gr) {
 #pragma unroll
-      for (int c = 0; c < kW4Part / 32; ++c) {
-        if (c % (GROUP / 32) == 0) {
+    for (int r = 0; r < 2 * MT; ++r) sc[r] = gr < groups ? __half_as_ushort(a.scales[at[r] + gr]) : 0u;
+  };
+  auto fetch_zero = [&](int gr, uint32_t (&z)[2 * MT]) {
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+    for (int r = 0; r < 2 * MT; ++r) z[r] = gr < groups ? a.zeros[at[r] + gr] : 8u;
+  };
+  fetch_scale(gr);
+  if constexpr (ZEROS) fetch_zero(gr, z);
+  // Up to eight batch rows: columns 8 t .. + 7 of each chunk of 32, of the row that is column g of the n-tile, straight
+  // into registers, a stage ahead. More: in the ring. Batch row 8 nt + xr is column g, so that the eight lanes of a
+  // 16-byte read's phase fall on all banks of the swizzled rows.
+  const int xr = (g & 1) * 4 + (g >> 1);
+  uint4 xs[NT == 1 ? CHUNKS : 1];
+  const __half* xsrc = a.x + (size_t)min(b0 + xr, a.B - 1) * a.K + s0 * C::KC + wk * kW4Part + 8 * t;
+  int xleft = b0 + xr < a.B && n_st > 0 ? a.K - s0 * C::KC - wk * kW4Part : 0;  // columns from xsrc's chunk on
+  if constexpr (NT == 1) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) d[mt][nt][0] = d[mt][nt][1] = d[mt][nt][2] = d[mt][nt][3] = 0.f;
-        }
-        const int gi = c / (GROUP / 32);  // group of the stage's GP
-        uint32_t w[4], h[2 * MT][4];
-        ldsm_x4(base_u + w_at + (((4 * (wk & 1) + c) ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+    for (int c = 0; c < CHUNKS; ++c)
+      xs[c] = 32 * c < xleft ? *reinterpret_cast<const uint4*>(xsrc + 32 * c) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  const uint32_t x_at = C::W_BYTES + wk * 2 * (8 * NT * 128) + xr * 128 + ((t ^ (xr & 3)) << 4);
+  // ldmatrix: row `lane` of the warp's 32, 16-byte chunk 4 (wk & 1) + c of its 128-byte row
+  const uint32_t w_at = (wk >> 1) * C::BM * 128 + (wm * 32 + lane) * 128;
+  const uint32_t w_swz = ((4 * (wk & 1)) ^ (lane & 7)) << 4;
+
+  bool ok = true;
+  float acc[MT][NT][4] = {};
+  int st = 0;
+  uint32_t parity = 0;
+#pragma unroll 1
+  for (int i = 0; i < n_st; ++i) {
+    ok = __all_sync(0xffffffffu, ok && wait(full + st, parity));
+    if (!ok) break;
+    if (tid == 0 && i > 0 && filled < n_st) {  // the stage before this one, once all warps have left it
+      ok = wait(empty + (st == 0 ? C::STAGES - 1 : st - 1), st == 0 ? parity ^ 1 : parity);
+      if (ok) fill(filled++);
+    }
+    gr += C::KC / GROUP;
+    xsrc += C::KC;
+    xleft -= C::KC;
+    uint32_t z1[2 * MT];
+    if constexpr (ZEROS) fetch_zero(i + 1 < n_st ? gr : groups, z1);
+    const uint8_t* base = smem + st * C::STAGE;
+    const uint32_t base_w = smem_u32(base) + w_at;
+    uint32_t z1024[2 * MT], z64[2 * MT];
+    float d[MT][NT][4];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      if (c % CG == 0) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) d[mt][nt][0] = d[mt][nt][1] = d[mt][nt][2] = d[mt][nt][3] = 0.f;
 #pragma unroll
         for (int r = 0; r < 2 * MT; ++r) {
-          const uint32_t zr = GP == 1 ? z[r] : __shfl_sync(0xffffffffu, z[r], (lane & ~3) + gi);
-          const uint32_t z1024 = (0x6400u + zr) * 0x10001u;
-          codes_less(w[r], z1024, h2_sub(0x63806380u, z1024), h[r]);  // 960 - (1024 + z)
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const uint4 x = *reinterpret_cast<const uint4*>(
-              base + ((x_at + (c >> 1) * (8 * NT * 128) + nt * 1024) ^ (((xr & 4) ^ (4 * (c & 1))) << 4)));
-          // columns 0..7 into the codes' order of pairs
-          const uint32_t p04 = __byte_perm(x.x, x.z, 0x5410), p15 = __byte_perm(x.x, x.z, 0x7632);
-          const uint32_t p26 = __byte_perm(x.y, x.w, 0x5410), p37 = __byte_perm(x.y, x.w, 0x7632);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            mma16816(d[mt][nt], h[2 * mt][0], h[2 * mt + 1][0], h[2 * mt][1], h[2 * mt + 1][1], p04, p15);
-            mma16816(d[mt][nt], h[2 * mt][2], h[2 * mt + 1][2], h[2 * mt][3], h[2 * mt + 1][3], p26, p37);
-          }
-        }
-        if ((c + 1) % (GROUP / 32) == 0) {
-#pragma unroll
-          for (int r = 0; r < 2 * MT; ++r) {
-            const uint32_t sr = GP == 1 ? sc[r] : __shfl_sync(0xffffffffu, sc[r], (lane & ~3) + gi);
-            const float f = __half2float(__ushort_as_half(uint16_t(sr)));
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              float* dst = acc[r >> 1][nt] + 2 * (r & 1);
-              const float* src = d[r >> 1][nt] + 2 * (r & 1);
-              dst[0] += f * src[0];
-              dst[1] += f * src[1];
-            }
+          if constexpr (ZEROS) {
+            const uint32_t zr = GP == 1 ? z[r] : __shfl_sync(0xffffffffu, z[r], (lane & ~3) + c / CG);
+            z1024[r] = (0x6400u + zr) * 0x10001u;
+            z64[r] = h2_sub(0x63806380u, z1024[r]);  // 960 - (1024 + z)
+          } else {
+            z1024[r] = 0x64086408u;  // 1032
+            z64[r] = 0xd480d480u;    // -72
           }
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(empty + st);
+      uint32_t w[4], h[2 * MT][4];
+      ldsm_x4(base_w + (w_swz ^ (c << 4)), w[0], w[1], w[2], w[3]);
 #pragma unroll
-      for (int r = 0; r < 2 * MT; ++r) {
-        sc[r] = sc1[r];
-        z[r] = z1[r];
+      for (int r = 0; r < 2 * MT; ++r) codes_less(w[r], z1024[r], z64[r], h[r]);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        uint4 x;
+        if constexpr (NT == 1) x = xs[c];
+        else
+          x = *reinterpret_cast<const uint4*>(
+              base + ((x_at + (c >> 1) * (8 * NT * 128) + nt * 1024) ^ (((xr & 4) ^ (4 * (c & 1))) << 4)));
+        // columns 0..7 into the codes' order of pairs
+        const uint32_t p04 = __byte_perm(x.x, x.z, 0x5410), p15 = __byte_perm(x.x, x.z, 0x7632);
+        const uint32_t p26 = __byte_perm(x.y, x.w, 0x5410), p37 = __byte_perm(x.y, x.w, 0x7632);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          mma16816(d[mt][nt], h[2 * mt][0], h[2 * mt + 1][0], h[2 * mt][1], h[2 * mt + 1][1], p04, p15);
+          mma16816(d[mt][nt], h[2 * mt][2], h[2 * mt + 1][2], h[2 * mt][3], h[2 * mt + 1][3], p26, p37);
+        }
+      }
+      if constexpr (NT == 1)
+        xs[c] = 32 * c < xleft && i + 1 < n_st ? *reinterpret_cast<const uint4*>(xsrc + 32 * c) : make_uint4(0u, 0u, 0u, 0u);
+      if ((c + 1) % CG == 0) {
+#pragma unroll
+        for (int r = 0; r < 2 * MT; ++r) {
+          const uint32_t sr = GP == 1 ? sc[r] : __shfl_sync(0xffffffffu, sc[r], (lane & ~3) + c / CG);
+          const float f = __half2float(__ushort_as_half(uint16_t(sr)));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float* dst = acc[r >> 1][nt] + 2 * (r & 1);
+            const float* src = d[r >> 1][nt] + 2 * (r & 1);
+            dst[0] += f * src[0];
+            dst[1] += f * src[1];
+          }
+        }
       }
     }
-    ok = __all_sync(0xffffffffu, ok);
-    if (!ok)
+    fetch_scale(i + 1 < n_st ? gr : groups);
+    if constexpr (ZEROS) {
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) acc[mt][nt][0] = acc[mt][nt][1] = acc[mt][nt][2] = acc[mt][nt][3] = __uint_as_float(0x7fc00000u);
+      for (int r = 0; r < 2 * MT; ++r) z[r] = z1[r];
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty + st);
+    st = st + 1 == C::STAGES ? 0 : st + 1;
+    parity ^= st == 0 ? 1u : 0u;
   }
+  ok = __all_sync(0xffffffffu, ok);
+  if (!ok)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) acc[mt][nt][0] = acc[mt][nt][1] = acc[mt][nt][2] = acc[mt][nt][3] = __uint_as_float(0x7fc00000u);
   // a CTA whose wait ran out still has copies on their way into the ring: wait for them (again with a limit)
   if (!__syncthreads_and(ok)) {
     if (tid == 0)
@@ -218,7 +257,7 @@ __global__ void __launch_bounds__(kW4Threads, W4Cfg<NT>::CTAS)
         part[(wk * 8 * NT + nt * 8 + t + 4 * (e & 1)) * C::BM + wm * 16 * MT + mt * 16 + g + 8 * (e >> 1)] = acc[mt][nt][e];
   __syncthreads();
   const int nb = min(8 * NT, a.B - b0);
-  for (int i = tid; i < nb * C::BM; i += kW4Threads) {
+  for (int i = tid; i < nb * C::BM; i += C::THREADS) {
     float sum = 0.f;
 #pragma unroll
     for (int k = 0; k < C::WK; ++k) sum += part[k * 8 * NT * C::BM + i];
@@ -230,7 +269,7 @@ __global__ void __launch_bounds__(kW4Threads, W4Cfg<NT>::CTAS)
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   const uint32_t joined_u = smem_u32(joined);
-  for (int i = rank * kW4Threads + tid; i < nb * C::BM; i += parts * kW4Threads) {
+  for (int i = rank * C::THREADS + tid; i < nb * C::BM; i += parts * C::THREADS) {
     float sum = 0.f;
 #pragma unroll 4
     for (int p = 0; p < parts; ++p) {
@@ -262,7 +301,7 @@ EncodeFn encode_fn() {
   return fn;
 }
 
-template <int NT, int GROUP>
+template <int NT, int GROUP, bool ZEROS>
 cudaError_t launch(const W4Args& a, int sms, cudaStream_t s) {
   using C = W4Cfg<NT>;
   const EncodeFn fn = encode_fn();
@@ -294,24 +333,33 @@ cudaError_t launch(const W4Args& a, int sms, cudaStream_t s) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((a.N + C::BM - 1) / C::BM * parts, (a.B + 8 * NT - 1) / (8 * NT));
-  cfg.blockDim = dim3(kW4Threads);
+  cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, w4_projection_kernel<NT, GROUP>, a, parts, wmap, xmap);
+  return cudaLaunchKernelEx(&cfg, w4_projection_kernel<NT, GROUP, ZEROS>, a, parts, wmap, xmap);
 }
 
+template <int NT, int GROUP>
+cudaError_t launch_group(const W4Args& a, int sms, cudaStream_t s) {
+  return a.zeros ? launch<NT, GROUP, true>(a, sms, s) : launch<NT, GROUP, false>(a, sms, s);
+}
 template <int NT>
 cudaError_t launch_nt(const W4Args& a, int sms, cudaStream_t s) {
-  return a.group == 32 ? launch<NT, 32>(a, sms, s) : a.group == 64 ? launch<NT, 64>(a, sms, s) : launch<NT, 128>(a, sms, s);
+  return a.group == 32   ? launch_group<NT, 32>(a, sms, s)
+         : a.group == 64 ? launch_group<NT, 64>(a, sms, s)
+                         : launch_group<NT, 128>(a, sms, s);
 }
 
+template <int NT, int GROUP>
+cudaError_t attrs_group() {
+  const cudaError_t e = set_kernel_smem(w4_projection_kernel<NT, GROUP, false>, W4Cfg<NT>::SMEM);
+  return e != cudaSuccess ? e : set_kernel_smem(w4_projection_kernel<NT, GROUP, true>, W4Cfg<NT>::SMEM);
+}
 template <int NT>
 cudaError_t attrs() {
-  for (const cudaError_t e : {set_kernel_smem(w4_projection_kernel<NT, 32>, W4Cfg<NT>::SMEM),
-                              set_kernel_smem(w4_projection_kernel<NT, 64>, W4Cfg<NT>::SMEM),
-                              set_kernel_smem(w4_projection_kernel<NT, 128>, W4Cfg<NT>::SMEM)})
+  for (const cudaError_t e : {attrs_group<NT, 32>(), attrs_group<NT, 64>(), attrs_group<NT, 128>()})
     if (e != cudaSuccess) return e;
   return cudaSuccess;
 }

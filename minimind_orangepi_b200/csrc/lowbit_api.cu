@@ -228,6 +228,7 @@ int mmc_op_w4_projection(int32_t batch, int32_t n, int32_t k, int32_t group, con
     require(batch >= 1 && batch <= 65535 && n >= 1 && k >= 1, "batch (at most 65535), n and k must be at least 1");
     require(group == 32 || group == 64 || group == 128, "group must be 32, 64 or 128");
     require(k % group == 0, "k must be a multiple of group");
+    require(n <= (1 << 30) && (int64_t)n * (k / group) < (int64_t(1) << 32), "n or n * (k / group) is too large");
     require(d_codes && d_scales_fp16 && d_x_fp16 && d_y, "null argument");
     require(aligned(d_codes, 16) && aligned(d_x_fp16, 16) && aligned(d_y, 16) && aligned(d_scales_fp16, 2),
             "d_codes, d_x and d_y must be 16-byte aligned");
