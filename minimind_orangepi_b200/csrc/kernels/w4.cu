@@ -13,6 +13,8 @@
 #include "common.cuh"
 #include "lowbit.h"
 
+#include <algorithm>
+
 namespace mmc {
 namespace {
 
@@ -20,15 +22,13 @@ constexpr int kW4Part = 128;                     // columns of a stage that one 
 
 template <int NT>
 struct W4Cfg {
-  static constexpr int WARPS = NT == 1 || NT == 8 ? 8 : 16, THREADS = WARPS * 32;
+  static constexpr int WARPS = NT == 8 ? 8 : 16, THREADS = WARPS * 32;
   static constexpr int MT = 2;                                   // 16-row tiles of a warp
-  static constexpr int WM = NT == 1 ? 1 : 4;                     // warps down the rows
+  static constexpr int WM = 4;                                   // warps down the rows
   static constexpr int WK = WARPS / WM;                          // warps along the columns
   static constexpr int BM = 16 * MT * WM, KC = kW4Part * WK;     // rows of a CTA, columns of a stage
-  // up to eight batch rows are read by the lanes that need them; more go through the ring
-  static constexpr int W_BYTES = BM * KC / 2, X_BYTES = NT == 1 ? 0 : 8 * NT * KC * 2, STAGE = W_BYTES + X_BYTES;
-  static constexpr int CTAS = NT == 1 ? 2 : 1;                   // of an SM
-  static constexpr int STAGES = 208 * 1024 / CTAS / STAGE;
+  static constexpr int W_BYTES = BM * KC / 2, X_BYTES = 8 * NT * KC * 2, STAGE = W_BYTES + X_BYTES;
+  static constexpr int STAGES = 208 * 1024 / STAGE;
   static constexpr int JOIN = (WK + 1) * BM * 8 * NT * 4;
   static constexpr int RING = STAGE * STAGES > JOIN ? STAGE * STAGES : JOIN;
   static constexpr int SMEM = 1024 + RING + 2 * STAGES * 8;
@@ -66,12 +66,24 @@ __device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, in
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
       : "memory");
 }
+__device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
+  uint32_t at;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+
 // A wait that a copy or a warp of this CTA ends; after two seconds it gives up
 // and the call's outputs become NaN (there is no error word to set).
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, nullptr); }
 
 template <int NT, int GROUP, bool ZEROS>
-__global__ void __launch_bounds__(W4Cfg<NT>::THREADS, W4Cfg<NT>::CTAS)
+__global__ void __launch_bounds__(W4Cfg<NT>::THREADS, 1)
     w4_projection_kernel(const W4Args a, int parts, const __grid_constant__ CUtensorMap wmap,
                          const __grid_constant__ CUtensorMap xmap) {
   using C = W4Cfg<NT>;
@@ -100,11 +112,9 @@ __global__ void __launch_bounds__(W4Cfg<NT>::THREADS, W4Cfg<NT>::CTAS)
     mbar_arrive_expect_tx(full + st, C::STAGE);
 #pragma unroll
     for (int j = 0; j < C::KC / 256; ++j) load_2d(dst + j * C::BM * 128, &wmap, s * (C::KC / 2) + j * 128, n0, full + st);
-    if constexpr (NT > 1) {
 #pragma unroll
-      for (int j = 0; j < C::KC / 64; ++j)
-        load_2d(dst + C::W_BYTES + j * 8 * NT * 128, &xmap, s * C::KC + j * 64, b0, full + st);
-    }
+    for (int j = 0; j < C::KC / 64; ++j)
+      load_2d(dst + C::W_BYTES + j * 8 * NT * 128, &xmap, s * C::KC + j * 64, b0, full + st);
   };
   int filled = min(C::STAGES, n_st);
   if (tid == 0)
@@ -119,7 +129,7 @@ __global__ void __launch_bounds__(W4Cfg<NT>::THREADS, W4Cfg<NT>::CTAS)
   for (int r = 0; r < 2 * MT; ++r) at[r] = min(n0 + wm * 32 + g + 8 * r, a.N - 1) * uint32_t(groups);
   int gr = s0 * (C::KC / GROUP) + wk * GP + t % GP;
   uint32_t sc[2 * MT], z[2 * MT];
-  auto fetch_scale = [&](int gr) {
+  auto fetch_scale = [&](int gr, uint32_t (&sc)[2 * MT]) {
 #pragma unroll
     for (int r = 0; r < 2 * MT; ++r) sc[r] = gr < groups ? __half_as_ushort(a.scales[at[r] + gr]) : 0u;
   };
@@ -127,20 +137,11 @@ __global__ void __launch_bounds__(W4Cfg<NT>::THREADS, W4Cfg<NT>::CTAS)
 #pragma unroll
     for (int r = 0; r < 2 * MT; ++r) z[r] = gr < groups ? a.zeros[at[r] + gr] : 8u;
   };
-  fetch_scale(gr);
+  fetch_scale(gr, sc);
   if constexpr (ZEROS) fetch_zero(gr, z);
-  // Up to eight batch rows: columns 8 t .. + 7 of each chunk of 32, of the row that is column g of the n-tile, straight
-  // into registers, a stage ahead. More: in the ring. Batch row 8 nt + xr is column g, so that the eight lanes of a
-  // 16-byte read's phase fall on all banks of the swizzled rows.
+  // Batch row 8 nt + xr is column g of an n-tile, so that the eight lanes of a 16-byte read's phase fall on all banks of the
+  // swizzled rows.
   const int xr = (g & 1) * 4 + (g >> 1);
-  uint4 xs[NT == 1 ? CHUNKS : 1];
-  const __half* xsrc = a.x + (size_t)min(b0 + xr, a.B - 1) * a.K + s0 * C::KC + wk * kW4Part + 8 * t;
-  int xleft = b0 + xr < a.B && n_st > 0 ? a.K - s0 * C::KC - wk * kW4Part : 0;  // columns from xsrc's chunk on
-  if constexpr (NT == 1) {
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c)
-      xs[c] = 32 * c < xleft ? *reinterpret_cast<const uint4*>(xsrc + 32 * c) : make_uint4(0u, 0u, 0u, 0u);
-  }
   const uint32_t x_at = C::W_BYTES + wk * 2 * (8 * NT * 128) + xr * 128 + ((t ^ (xr & 3)) << 4);
   // ldmatrix: row `lane` of the warp's 32, 16-byte chunk 4 (wk & 1) + c of its 128-byte row
   const uint32_t w_at = (wk >> 1) * C::BM * 128 + (wm * 32 + lane) * 128;
@@ -159,9 +160,13 @@ __global__ void __launch_bounds__(W4Cfg<NT>::THREADS, W4Cfg<NT>::CTAS)
       if (ok) fill(filled++);
     }
     gr += C::KC / GROUP;
-    xsrc += C::KC;
-    xleft -= C::KC;
-    uint32_t z1[2 * MT];
+    if (i + 3 < n_st) {  // the scales of three stages on, into L2
+      const size_t far = (size_t)min(n0 + wm * 32 + lane, a.N - 1) * groups + min(gr - t % GP + 2 * (C::KC / GROUP), groups - 1);
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(a.scales + far));
+      if constexpr (ZEROS) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.zeros + far));
+    }
+    uint32_t sc1[2 * MT], z1[2 * MT];
+    fetch_scale(i + 1 < n_st ? gr : groups, sc1);
     if constexpr (ZEROS) fetch_zero(i + 1 < n_st ? gr : groups, z1);
     const uint8_t* base = smem + st * C::STAGE;
     const uint32_t base_w = smem_u32(base) + w_at;
@@ -192,11 +197,8 @@ __global__ void __launch_bounds__(W4Cfg<NT>::THREADS, W4Cfg<NT>::CTAS)
       for (int r = 0; r < 2 * MT; ++r) codes_less(w[r], z1024[r], z64[r], h[r]);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        uint4 x;
-        if constexpr (NT == 1) x = xs[c];
-        else
-          x = *reinterpret_cast<const uint4*>(
-              base + ((x_at + (c >> 1) * (8 * NT * 128) + nt * 1024) ^ (((xr & 4) ^ (4 * (c & 1))) << 4)));
+        const uint4 x = *reinterpret_cast<const uint4*>(
+            base + ((x_at + (c >> 1) * (8 * NT * 128) + nt * 1024) ^ (((xr & 4) ^ (4 * (c & 1))) << 4)));
         // columns 0..7 into the codes' order of pairs
         const uint32_t p04 = __byte_perm(x.x, x.z, 0x5410), p15 = __byte_perm(x.x, x.z, 0x7632);
         const uint32_t p26 = __byte_perm(x.y, x.w, 0x5410), p37 = __byte_perm(x.y, x.w, 0x7632);
@@ -206,8 +208,6 @@ __global__ void __launch_bounds__(W4Cfg<NT>::THREADS, W4Cfg<NT>::CTAS)
           mma16816(d[mt][nt], h[2 * mt][2], h[2 * mt + 1][2], h[2 * mt][3], h[2 * mt + 1][3], p26, p37);
         }
       }
-      if constexpr (NT == 1)
-        xs[c] = 32 * c < xleft && i + 1 < n_st ? *reinterpret_cast<const uint4*>(xsrc + 32 * c) : make_uint4(0u, 0u, 0u, 0u);
       if ((c + 1) % CG == 0) {
 #pragma unroll
         for (int r = 0; r < 2 * MT; ++r) {
@@ -223,10 +223,10 @@ __global__ void __launch_bounds__(W4Cfg<NT>::THREADS, W4Cfg<NT>::CTAS)
         }
       }
     }
-    fetch_scale(i + 1 < n_st ? gr : groups);
-    if constexpr (ZEROS) {
 #pragma unroll
-      for (int r = 0; r < 2 * MT; ++r) z[r] = z1[r];
+    for (int r = 0; r < 2 * MT; ++r) {
+      sc[r] = sc1[r];
+      if constexpr (ZEROS) z[r] = z1[r];
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(empty + st);
@@ -266,24 +266,253 @@ __global__ void __launch_bounds__(W4Cfg<NT>::THREADS, W4Cfg<NT>::CTAS)
     else if (n < a.N) a.y[(size_t)(b0 + i / C::BM) * a.N + n] = sum;
   }
   if (parts == 1) return;
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_barrier();
   const uint32_t joined_u = smem_u32(joined);
   for (int i = rank * C::THREADS + tid; i < nb * C::BM; i += parts * C::THREADS) {
     float sum = 0.f;
 #pragma unroll 4
-    for (int p = 0; p < parts; ++p) {
-      uint32_t at;
-      float v;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(joined_u + 4 * i), "r"(p));
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-      sum += v;
-    }
+    for (int p = 0; p < parts; ++p) sum += ld_cluster(joined_u + 4 * i, p);
     const int n = n0 + i % C::BM;
     if (n < a.N) a.y[(size_t)(b0 + i / C::BM) * a.N + n] = sum;
   }
-  __syncwarp();  // no CTA leaves while another reads its shared memory
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_barrier();  // no CTA leaves while another reads its shared memory
+}
+
+// Up to eight batch rows: bound by HBM, so each SM gets one CTA with an even share
+// of the 16-row tiles, one pass over the columns and one join at its end. WM warps
+// down the rows and WK along the columns, PART columns of each stage a warp. With
+// so few rows the instructions that take the codes to the tensor core count: x is
+// laid out once in shared memory in the codes' order of pairs (XS), where it has
+// room, and read from L1 or L2 otherwise.
+struct W4RowsPlan {
+  int wm, wk, stages, parts, per;  // parts: CTAs of a cluster that share the columns, `per` stages each
+  int ring;                        // bytes
+};
+constexpr int kW4RowsWarps = 16;
+constexpr int kW4RowsSmem = 224 * 1024, kW4RowsHead = 1024;  // barriers, alignment
+constexpr int kW4RowsX = 96 * 1024;                          // most of x in shared memory
+
+// D = A * B (no sum goes in)
+__device__ __forceinline__ void mma16816_zero(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                              uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+template <int PART, int GROUP, bool ZEROS, bool XS>
+__global__ void __launch_bounds__(32 * kW4RowsWarps, 1)
+    w4_rows_kernel(const W4Args a, const W4RowsPlan p, const __grid_constant__ CUtensorMap wmap) {
+  constexpr int SUBS = PART / 128, CG = GROUP / 32, SG = 128 / GROUP;  // runs of 128 columns, chunks of a group, groups of a run
+  constexpr int PG = PART / GROUP;                                     // groups of a part:
+  constexpr bool EACH = PG <= 2;                                       // every lane reads its rows' or, with more, one in four
+  constexpr int LG = EACH ? PG : PG / 4;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  __shared__ uint64_t full[32], empty[32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  uint32_t rank;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int rows = 16 * p.wm, kc = PART * p.wk, stage_bytes = rows * kc / 2;
+  const int n0 = blockIdx.x / p.parts * rows;
+  const int all = (a.K + kc - 1) / kc;
+  const int s0 = min(all, int(rank) * p.per), n_st = min(all, s0 + p.per) - s0;
+  if (tid < p.stages) {
+    mbar_init(full + tid, 1);
+    mbar_init(empty + tid, p.wm * p.wk);
+  }
+  fence_mbar_init();
+  __syncthreads();
+  int filled = 0;  // thread 0: stages whose copies have started
+  auto fill = [&](int st) {
+    const uint32_t dst = smem_u32(smem + st * stage_bytes);
+    mbar_arrive_expect_tx(full + st, stage_bytes);
+    for (int j = 0; j < kc / 256; ++j)
+      load_2d(dst + j * rows * 128, &wmap, (s0 + filled) * (kc / 2) + j * 128, n0, full + st);
+    ++filled;
+  };
+  if (tid == 0)
+    while (filled < min(p.stages, n_st)) fill(filled);
+
+  const int wm = warp % p.wm, wk = warp / p.wm;
+  const int groups = a.K / GROUP;
+  uint32_t at[2];  // scale rows (behind N: the last one's, not stored)
+#pragma unroll
+  for (int r = 0; r < 2; ++r) at[r] = min(n0 + wm * 16 + g + 8 * r, a.N - 1) * uint32_t(groups);
+  const int xr = min((g & 1) * 4 + (g >> 1), a.B - 1);  // the batch row that is column g (as above); behind the batch: the last, not stored
+  const uint32_t pitch = p.per * kc * 2 + 16;           // of a row of x in shared memory: rows r and r + 4 half the banks apart
+  uint8_t* xsm = smem + p.ring;
+  if constexpr (XS) {
+    const int cols = n_st * kc / 8;
+    for (int b = 0; b < a.B; ++b)
+      for (int c0 = tid; c0 < cols; c0 += 4 * blockDim.x) {
+        uint4 x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int c = c0 + u * blockDim.x;
+          x[u] = c < cols && s0 * kc + 8 * c < a.K ? *reinterpret_cast<const uint4*>(a.x + (size_t)b * a.K + s0 * kc + 8 * c)
+                                                   : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int c = c0 + u * blockDim.x;
+          if (c < cols)
+            *reinterpret_cast<uint4*>(xsm + b * pitch + 16 * c) =
+                make_uint4(__byte_perm(x[u].x, x[u].z, 0x5410), __byte_perm(x[u].x, x[u].z, 0x7632),
+                           __byte_perm(x[u].y, x[u].w, 0x5410), __byte_perm(x[u].y, x[u].w, 0x7632));
+        }
+      }
+  }
+  // ldmatrix: row (lane & 15) of the warp's 16, 16-byte chunks c and c + 1 of its part
+  const uint32_t w_lane = (wk * PART >> 8) * rows * 128 + (wm * 16 + (lane & 15)) * 128 +
+                          ((((lane >> 4) ^ (lane & 7)) << 4) ^ ((wk * PART & 128) >> 1));
+  const uint8_t* x_lane = xsm + xr * pitch + wk * PART * 2 + 16 * t;
+  const __half* xrow = a.x + (size_t)xr * a.K + 8 * t;
+  uint4 xs[XS ? 1 : 4];
+  uint32_t sc[2][LG], z[2][LG];
+  auto fetch_scales = [&](int k, uint32_t (&sc)[2][LG], uint32_t (&z)[2][LG]) {
+#pragma unroll
+    for (int j = 0; j < LG; ++j) {
+      const int gr = k / GROUP + (EACH ? j : 4 * j + t);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        sc[r][j] = gr < groups ? __half_as_ushort(a.scales[at[r] + gr]) : 0u;
+        if constexpr (ZEROS) z[r][j] = gr < groups ? a.zeros[at[r] + gr] : 8u;
+      }
+    }
+  };
+  int k = s0 * kc + wk * PART;  // this warp's first column of the stage
+  fetch_scales(k, sc, z);
+  if constexpr (!XS) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) xs[c] = k + 32 * c < a.K ? *reinterpret_cast<const uint4*>(xrow + k + 32 * c) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  if constexpr (XS) __syncthreads();
+  bool ok = true;
+  int st = 0;
+  uint32_t parity = 0;
+  float acc[4] = {};
+#pragma unroll 1
+  for (int i = 0; i < n_st; ++i) {
+    uint32_t sc1[2][LG], z1[2][LG];
+    if (i + 4 < n_st && lane < 16) {  // the scales of four stages on, into L2
+      const uint32_t far = min(n0 + wm * 16 + lane, a.N - 1) * uint32_t(groups) + min((k + 4 * kc) / GROUP, groups - 1);
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(a.scales + far));
+      if constexpr (ZEROS) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.zeros + far));
+    }
+    fetch_scales(k + kc, sc1, z1);
+    ok = __all_sync(0xffffffffu, ok && wait(full + st, parity));
+    if (!ok) break;
+    if (tid == 0 && i > 0 && filled < n_st) {  // the stage before this one, once all warps have left it
+      const int before = st == 0 ? p.stages - 1 : st - 1;
+      ok = wait(empty + before, st == 0 ? parity ^ 1 : parity);
+      if (ok) fill(before);
+    }
+    const uint32_t w_st = smem_u32(smem) + st * stage_bytes + w_lane;
+#pragma unroll
+    for (int sub = 0; sub < SUBS; ++sub) {
+      const uint32_t w_at = PART == 128 ? w_st : (w_st + (sub >> 1) * rows * 128) ^ ((sub & 1) << 6);
+      uint32_t z1024[2], z64[2], w[4];
+      float d[4], e[4];  // two chains of products
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int j = sub * SG + c / CG;  // group of the part
+        if (c % CG == 0) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            if constexpr (ZEROS) {
+              const uint32_t zr = EACH ? z[r][j % LG] : __shfl_sync(0xffffffffu, z[r][(j / 4) % LG], (lane & ~3) + j % 4);
+              z1024[r] = (0x6400u + zr) * 0x10001u;
+              z64[r] = h2_sub(0x63806380u, z1024[r]);  // 960 - (1024 + z)
+            } else {
+              z1024[r] = 0x64086408u;  // 1032
+              z64[r] = 0xd480d480u;    // -72
+            }
+          }
+        }
+        if (c % 2 == 0) ldsm_x4(w_at ^ (c << 4), w[0], w[1], w[2], w[3]);
+        uint32_t h0[4], h1[4];
+        codes_less(w[2 * (c & 1)], z1024[0], z64[0], h0);
+        codes_less(w[2 * (c & 1) + 1], z1024[1], z64[1], h1);
+        uint4 x;
+        if constexpr (XS) {
+          x = *reinterpret_cast<const uint4*>(x_lane + sub * 256 + c * 64);
+        } else {
+          const uint4 y = xs[c];
+          x = make_uint4(__byte_perm(y.x, y.z, 0x5410), __byte_perm(y.x, y.z, 0x7632), __byte_perm(y.y, y.w, 0x5410),
+                         __byte_perm(y.y, y.w, 0x7632));
+        }
+        if (c % CG == 0) {
+          mma16816_zero(d, h0[0], h1[0], h0[1], h1[1], x.x, x.y);
+          mma16816_zero(e, h0[2], h1[2], h0[3], h1[3], x.z, x.w);
+        } else {
+          mma16816(d, h0[0], h1[0], h0[1], h1[1], x.x, x.y);
+          mma16816(e, h0[2], h1[2], h0[3], h1[3], x.z, x.w);
+        }
+        if constexpr (!XS) {
+          const int kn = k + (sub + 1 < SUBS ? 128 * (sub + 1) : kc) + 32 * c;  // the next run's chunk
+          xs[c] = kn < a.K ? *reinterpret_cast<const uint4*>(xrow + kn) : make_uint4(0u, 0u, 0u, 0u);
+        }
+        if ((c + 1) % CG == 0) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t sr = EACH ? sc[r][j % LG] : __shfl_sync(0xffffffffu, sc[r][(j / 4) % LG], (lane & ~3) + j % 4);
+            const float f = __half2float(__ushort_as_half(uint16_t(sr)));
+            acc[2 * r] += f * (d[2 * r] + e[2 * r]);
+            acc[2 * r + 1] += f * (d[2 * r + 1] + e[2 * r + 1]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty + st);
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int j = 0; j < LG; ++j) {
+        sc[r][j] = sc1[r][j];
+        if constexpr (ZEROS) z[r][j] = z1[r][j];
+      }
+    k += kc;
+    x_lane += 2 * kc;
+    st = st + 1 == p.stages ? 0 : st + 1;
+    parity ^= st == 0 ? 1u : 0u;
+  }
+  // after a wait that ran out: outputs are NaN, and no copy may be on its way when the CTA goes on (waits have a limit)
+  if (!__syncthreads_and(ok)) {
+    acc[0] = acc[1] = acc[2] = acc[3] = __uint_as_float(0x7fc00000u);
+    if (tid == 0)
+      for (int i = max(0, filled - p.stages); i < filled; ++i) wait(full + i % p.stages, (i / p.stages) & 1);
+    __syncthreads();
+  }
+  // ---- join the warps along the columns, then the cluster's CTAs
+  float4* part = reinterpret_cast<float4*>(smem);                              // [wk][wm][lane]
+  float* joined = reinterpret_cast<float*>(part + p.wm * p.wk * 32);           // [wm][lane][4]
+  part[warp * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  __syncthreads();
+  auto store = [&](int i, float sum) {  // value e of lane l of row tile i / 128
+    const int l = (i >> 2) & 31, e = i & 3;
+    const int n = n0 + (i >> 7) * 16 + (l >> 2) + 8 * (e >> 1), b = (l & 3) + 4 * (e & 1);
+    if (n < a.N && b < a.B) a.y[(size_t)b * a.N + n] = sum;
+  };
+  const float* src = reinterpret_cast<const float*>(part);
+  for (int i = tid; i < p.wm * 128; i += blockDim.x) {
+    float sum = 0.f;
+    for (int w = 0; w < p.wk; ++w) sum += src[w * p.wm * 128 + i];
+    if (p.parts > 1) joined[i] = sum;
+    else store(i, sum);
+  }
+  if (p.parts == 1) return;
+  cluster_barrier();
+  const uint32_t joined_u = smem_u32(joined);
+  for (int i = rank * blockDim.x + tid; i < p.wm * 128; i += p.parts * blockDim.x) {
+    float sum = 0.f;
+#pragma unroll 4
+    for (int r = 0; r < p.parts; ++r) sum += ld_cluster(joined_u + 4 * i, r);
+    store(i, sum);
+  }
+  cluster_barrier();  // no CTA leaves while another reads its shared memory
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -301,32 +530,72 @@ EncodeFn encode_fn() {
   return fn;
 }
 
-template <int NT, int GROUP, bool ZEROS>
-cudaError_t launch(const W4Args& a, int sms, cudaStream_t s) {
-  using C = W4Cfg<NT>;
+// codes [N][K / 2] bytes, boxes of 128 bytes x `rows`; x [B][K] fp16, boxes of 64 columns x `rows`; 128-byte swizzle
+cudaError_t make_map(CUtensorMap* m, CUtensorMapDataType type, const void* base, int64_t cols, int64_t rows, int64_t pitch,
+                     int box_cols, int box_rows) {
   const EncodeFn fn = encode_fn();
   if (!fn) return cudaErrorNotSupported;
+  const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)}, strides[1] = {cuuint64_t(pitch)};
+  const cuuint32_t box[2] = {cuuint32_t(box_cols), cuuint32_t(box_rows)}, one[2] = {1, 1};
+  const CUresult r = fn(m, type, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+template <int PART, int GROUP, bool ZEROS, bool XS>
+cudaError_t launch_rows_x(const W4Args& a, const W4RowsPlan& p, int ctas, cudaStream_t s) {
+  CUtensorMap wmap;
+  const cudaError_t e = make_map(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, a.K / 2, a.N, a.K / 2, 128, 16 * p.wm);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.parts;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas * p.parts);
+  cfg.blockDim = dim3(32 * p.wm * p.wk);
+  cfg.dynamicSmemBytes = kW4RowsSmem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.parts > 1 ? 1 : 0;  // (a cluster of one costs a launch some 0.3 us)
+  return cudaLaunchKernelEx(&cfg, w4_rows_kernel<PART, GROUP, ZEROS, XS>, a, p, wmap);
+}
+
+template <int PART, int GROUP, bool ZEROS>
+cudaError_t launch_rows(const W4Args& a, int sms, cudaStream_t s) {
+  const int tiles = (a.N + 15) / 16, k_parts = (a.K + PART - 1) / PART;
+  W4RowsPlan p;
+  // one round of the SMs where sixteen warps' tiles are enough, the other warps along the columns
+  p.wm = std::min(PART == 128 ? 8 : 16, (tiles + sms - 1) / sms);
+  p.wk = std::max(1, std::min(kW4RowsWarps / p.wm, k_parts));
+  if (PART == 128) p.wk = std::max(2, p.wk & ~1);  // (boxes of 256 columns)
+  const int ctas = (tiles + p.wm - 1) / p.wm, all = (k_parts + p.wk - 1) / p.wk;
+  p.parts = 1;  // while the SMs are not full, CTAs share the columns
+  while (p.parts < 8 && ctas * p.parts * 2 <= sms && all >= 2 * p.parts) p.parts *= 2;
+  p.per = (all + p.parts - 1) / p.parts;
+  const int64_t x_bytes = (int64_t)a.B * ((int64_t)p.per * PART * p.wk * 2 + 16);
+  const bool xs = PART > 128 && x_bytes <= kW4RowsX;
+  const int stage = 16 * p.wm * PART * p.wk / 2;
+  p.stages = int(std::min<int64_t>(32, (kW4RowsSmem - kW4RowsHead - (xs ? x_bytes : 0)) / stage));
+  p.ring = p.stages * stage;
+  return xs ? launch_rows_x<PART, GROUP, ZEROS, true>(a, p, ctas, s) : launch_rows_x<PART, GROUP, ZEROS, false>(a, p, ctas, s);
+}
+
+template <int NT, int GROUP, bool ZEROS>
+cudaError_t launch(const W4Args& a, int sms, cudaStream_t s) {
+  if constexpr (NT == 1) {
+    return a.K >= 2048 ? launch_rows<256, GROUP, ZEROS>(a, sms, s) : launch_rows<128, GROUP, ZEROS>(a, sms, s);
+  } else {
+  using C = W4Cfg<NT>;
   CUtensorMap wmap, xmap;
-  {  // codes [N][K / 2] bytes, boxes of 128 bytes x BM rows, 128-byte swizzle
-    const cuuint64_t dims[2] = {cuuint64_t(a.K / 2), cuuint64_t(a.N)}, strides[1] = {cuuint64_t(a.K / 2)};
-    const cuuint32_t box[2] = {128, C::BM}, one[2] = {1, 1};
-    if (fn(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(a.codes), dims, strides, box, one,
-           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-      return cudaErrorInvalidValue;
-  }
-  {  // x [B][K] fp16, boxes of 64 columns x 8 NT rows, 128-byte swizzle
-    const cuuint64_t dims[2] = {cuuint64_t(a.K), cuuint64_t(a.B)}, strides[1] = {cuuint64_t(a.K) * 2};
-    const cuuint32_t box[2] = {64, 8 * NT}, one[2] = {1, 1};
-    if (fn(&xmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<__half*>(a.x), dims, strides, box, one,
-           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-      return cudaErrorInvalidValue;
-  }
+  cudaError_t e = make_map(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, a.K / 2, a.N, a.K / 2, 128, C::BM);
+  if (e == cudaSuccess)
+    e = make_map(&xmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.x, a.K, a.B, (int64_t)a.K * 2, 64, 8 * NT);
+  if (e != cudaSuccess) return e;
   const int64_t tiles = (int64_t)((a.N + C::BM - 1) / C::BM) * ((a.B + 8 * NT - 1) / (8 * NT));
   const int stages = (a.K + C::KC - 1) / C::KC;
   int parts = 1;  // CTAs that share the columns: while they find places, and two stages each
-  while (parts < 8 && tiles * parts * 2 <= (int64_t)sms * C::CTAS && stages >= 4 * parts) parts *= 2;
+  while (parts < 8 && tiles * parts * 2 <= sms && stages >= 4 * parts) parts *= 2;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = parts;
@@ -337,8 +606,9 @@ cudaError_t launch(const W4Args& a, int sms, cudaStream_t s) {
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = parts > 1 ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, w4_projection_kernel<NT, GROUP, ZEROS>, a, parts, wmap, xmap);
+  }
 }
 
 template <int NT, int GROUP>
@@ -352,10 +622,23 @@ cudaError_t launch_nt(const W4Args& a, int sms, cudaStream_t s) {
                          : launch_group<NT, 128>(a, sms, s);
 }
 
+template <int NT, int GROUP, bool ZEROS>
+cudaError_t attrs_kernel() {
+  if constexpr (NT == 1) {
+    for (const cudaError_t e : {set_kernel_smem(w4_rows_kernel<128, GROUP, ZEROS, false>, kW4RowsSmem),
+                                set_kernel_smem(w4_rows_kernel<128, GROUP, ZEROS, true>, kW4RowsSmem),
+                                set_kernel_smem(w4_rows_kernel<256, GROUP, ZEROS, false>, kW4RowsSmem),
+                                set_kernel_smem(w4_rows_kernel<256, GROUP, ZEROS, true>, kW4RowsSmem)})
+      if (e != cudaSuccess) return e;
+    return cudaSuccess;
+  } else {
+    return set_kernel_smem(w4_projection_kernel<NT, GROUP, ZEROS>, W4Cfg<NT>::SMEM);
+  }
+}
 template <int NT, int GROUP>
 cudaError_t attrs_group() {
-  const cudaError_t e = set_kernel_smem(w4_projection_kernel<NT, GROUP, false>, W4Cfg<NT>::SMEM);
-  return e != cudaSuccess ? e : set_kernel_smem(w4_projection_kernel<NT, GROUP, true>, W4Cfg<NT>::SMEM);
+  const cudaError_t e = attrs_kernel<NT, GROUP, false>();
+  return e != cudaSuccess ? e : attrs_kernel<NT, GROUP, true>();
 }
 template <int NT>
 cudaError_t attrs() {
