@@ -28,10 +28,11 @@ struct W4Cfg {
   static constexpr int WK = WARPS / WM;                          // warps along the columns
   static constexpr int BM = 16 * MT * WM, KC = kW4Part * WK;     // rows of a CTA, columns of a stage
   static constexpr int W_BYTES = BM * KC / 2, X_BYTES = 8 * NT * KC * 2, STAGE = W_BYTES + X_BYTES;
-  static constexpr int STAGES = 208 * 1024 / STAGE;
+  static constexpr int SC_BYTES = BM * (KC / 32) * 3;            // scales and zero points of the smallest groups
+  static constexpr int STAGES = 216 * 1024 / (STAGE + SC_BYTES);
   static constexpr int JOIN = (WK + 1) * BM * 8 * NT * 4;
   static constexpr int RING = STAGE * STAGES > JOIN ? STAGE * STAGES : JOIN;
-  static constexpr int SMEM = 1024 + RING + 2 * STAGES * 8;
+  static constexpr int SMEM = 1024 + RING + STAGES * SC_BYTES + 2 * STAGES * 8;
 };
 
 __device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
@@ -66,6 +67,43 @@ __device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, in
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
       : "memory");
 }
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// One row's scales (and zero points) of a stage, groups gr0 .. gr0 + gps - 1, by
+// one thread: asynchronous copies as wide as the addresses allow, which arrive at
+// `bar` when they are done; groups behind the last one read as 0. An odd number
+// of groups a row leaves halves that such copies cannot take.
+template <bool ZEROS>
+__device__ __forceinline__ void copy_scales(const W4Args& a, uint8_t* sc, uint8_t* z, int row, int groups, int gr0, int gps,
+                                            uint64_t* bar) {
+  const size_t at = (size_t)row * groups + gr0;
+  const int have = min(max(groups - gr0, 0), gps);
+  auto copy = [&](uint8_t* dst, const uint8_t* src, int bytes, int valid, uint32_t align) {
+    if (align % 16 == 0) {
+      for (int o = 0; o < bytes; o += 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + o)),
+                     "l"(valid > o ? src + o : reinterpret_cast<const uint8_t*>(a.codes)), "r"(min(max(valid - o, 0), 16))
+                     : "memory");
+    } else if (align % 4 == 0) {
+      for (int o = 0; o < bytes; o += 4)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst + o)),
+                     "l"(valid > o ? src + o : reinterpret_cast<const uint8_t*>(a.codes)), "r"(min(max(valid - o, 0), 4))
+                     : "memory");
+    } else {
+      for (int o = 0; o < bytes; ++o) dst[o] = o < valid ? src[o] : 0;
+    }
+    return align % 4 == 0;
+  };
+  const uint8_t* s = reinterpret_cast<const uint8_t*>(a.scales);
+  bool async = copy(sc, s + 2 * at, 2 * gps, 2 * have, uint32_t(reinterpret_cast<uintptr_t>(s)) | 2 * groups | 2 * gps);
+  if constexpr (ZEROS)
+    async &= copy(z, a.zeros + at, gps, have, uint32_t(reinterpret_cast<uintptr_t>(a.zeros)) | groups | gps);
+  if (async) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+  } else {
+    cp_async_wait_all();
+    mbar_arrive(bar);
+  }
+}
 __device__ __forceinline__ void cluster_barrier() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -91,8 +129,10 @@ __global__ void __launch_bounds__(W4Cfg<NT>::THREADS, 1)
   constexpr int CG = GROUP / 32, GP = kW4Part / GROUP;  // 32-column chunks of a group, groups of a warp's part
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::RING);
+  uint8_t* scales = smem + C::RING;  // [stage][BM][GPS] fp16, [BM][GPS] bytes
+  uint64_t* full = reinterpret_cast<uint64_t*>(scales + C::STAGES * C::SC_BYTES);
   uint64_t* empty = full + C::STAGES;
+  constexpr int GPS = C::KC / GROUP;  // groups of a stage
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint32_t rank;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -100,45 +140,34 @@ __global__ void __launch_bounds__(W4Cfg<NT>::THREADS, 1)
   const int all = (a.K + C::KC - 1) / C::KC, per = (all + parts - 1) / parts;
   const int s0 = min(all, int(rank) * per), n_st = min(all, s0 + per) - s0;  // this CTA's stages of columns
   if (tid < C::STAGES) {
-    mbar_init(full + tid, 1);
+    mbar_init(full + tid, 1 + C::BM);
     mbar_init(empty + tid, C::WARPS);
   }
   fence_mbar_init();
   __syncthreads();
-  // thread 0 starts the copies of this CTA's i-th stage
+  // the first BM threads start the copies of this CTA's i-th stage: thread 0 codes and x, each its row's scales
+  const int groups = a.K / GROUP;
   auto fill = [&](int i) {
     const int s = s0 + i, st = i % C::STAGES;
-    const uint32_t dst = smem_u32(smem + st * C::STAGE);
-    mbar_arrive_expect_tx(full + st, C::STAGE);
+    if (tid == 0) {
+      const uint32_t dst = smem_u32(smem + st * C::STAGE);
+      mbar_arrive_expect_tx(full + st, C::STAGE);
 #pragma unroll
-    for (int j = 0; j < C::KC / 256; ++j) load_2d(dst + j * C::BM * 128, &wmap, s * (C::KC / 2) + j * 128, n0, full + st);
+      for (int j = 0; j < C::KC / 256; ++j) load_2d(dst + j * C::BM * 128, &wmap, s * (C::KC / 2) + j * 128, n0, full + st);
 #pragma unroll
-    for (int j = 0; j < C::KC / 64; ++j)
-      load_2d(dst + C::W_BYTES + j * 8 * NT * 128, &xmap, s * C::KC + j * 64, b0, full + st);
+      for (int j = 0; j < C::KC / 64; ++j)
+        load_2d(dst + C::W_BYTES + j * 8 * NT * 128, &xmap, s * C::KC + j * 64, b0, full + st);
+    }
+    uint8_t* sc = scales + st * C::SC_BYTES;
+    copy_scales<ZEROS>(a, sc + tid * GPS * 2, sc + C::BM * GPS * 2 + tid * GPS, min(n0 + tid, a.N - 1), groups, s * GPS, GPS, full + st);
   };
   int filled = min(C::STAGES, n_st);
-  if (tid == 0)
+  if (tid < C::BM)
     for (int i = 0; i < filled; ++i) fill(i);
 
   const int wm = warp % C::WM, wk = warp / C::WM;
-  // this lane's weight rows n0 + 32 wm + g + 8 r; of a stage's GP groups of this warp it fetches the (t % GP)-th, a stage
-  // ahead. (Rows behind N repeat the last one and are not stored; groups behind K have x = 0 and the scale 0.)
-  const int groups = a.K / GROUP;
-  uint32_t at[2 * MT];
-#pragma unroll
-  for (int r = 0; r < 2 * MT; ++r) at[r] = min(n0 + wm * 32 + g + 8 * r, a.N - 1) * uint32_t(groups);
-  int gr = s0 * (C::KC / GROUP) + wk * GP + t % GP;
-  uint32_t sc[2 * MT], z[2 * MT];
-  auto fetch_scale = [&](int gr, uint32_t (&sc)[2 * MT]) {
-#pragma unroll
-    for (int r = 0; r < 2 * MT; ++r) sc[r] = gr < groups ? __half_as_ushort(a.scales[at[r] + gr]) : 0u;
-  };
-  auto fetch_zero = [&](int gr, uint32_t (&z)[2 * MT]) {
-#pragma unroll
-    for (int r = 0; r < 2 * MT; ++r) z[r] = gr < groups ? a.zeros[at[r] + gr] : 8u;
-  };
-  fetch_scale(gr, sc);
-  if constexpr (ZEROS) fetch_zero(gr, z);
+  // this lane's weight rows of the CTA's are 32 wm + g + 8 r (behind N: the last one's scales, not stored)
+  const int sc_at = (wm * 32 + g) * GPS + wk * GP;
   // Batch row 8 nt + xr is column g of an n-tile, so that the eight lanes of a 16-byte read's phase fall on all banks of the
   // swizzled rows.
   const int xr = (g & 1) * 4 + (g >> 1);
@@ -155,19 +184,12 @@ __global__ void __launch_bounds__(W4Cfg<NT>::THREADS, 1)
   for (int i = 0; i < n_st; ++i) {
     ok = __all_sync(0xffffffffu, ok && wait(full + st, parity));
     if (!ok) break;
-    if (tid == 0 && i > 0 && filled < n_st) {  // the stage before this one, once all warps have left it
+    if (tid < C::BM && i > 0 && filled < n_st) {  // the stage before this one, once all warps have left it
       ok = wait(empty + (st == 0 ? C::STAGES - 1 : st - 1), st == 0 ? parity ^ 1 : parity);
       if (ok) fill(filled++);
     }
-    gr += C::KC / GROUP;
-    if (i + 3 < n_st) {  // the scales of three stages on, into L2
-      const size_t far = (size_t)min(n0 + wm * 32 + lane, a.N - 1) * groups + min(gr - t % GP + 2 * (C::KC / GROUP), groups - 1);
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(a.scales + far));
-      if constexpr (ZEROS) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.zeros + far));
-    }
-    uint32_t sc1[2 * MT], z1[2 * MT];
-    fetch_scale(i + 1 < n_st ? gr : groups, sc1);
-    if constexpr (ZEROS) fetch_zero(i + 1 < n_st ? gr : groups, z1);
+    const __half* sc_st = reinterpret_cast<const __half*>(scales + st * C::SC_BYTES) + sc_at;
+    const uint8_t* z_st = scales + st * C::SC_BYTES + C::BM * GPS * 2 + sc_at;
     const uint8_t* base = smem + st * C::STAGE;
     const uint32_t base_w = smem_u32(base) + w_at;
     uint32_t z1024[2 * MT], z64[2 * MT];
@@ -182,8 +204,7 @@ __global__ void __launch_bounds__(W4Cfg<NT>::THREADS, 1)
 #pragma unroll
         for (int r = 0; r < 2 * MT; ++r) {
           if constexpr (ZEROS) {
-            const uint32_t zr = GP == 1 ? z[r] : __shfl_sync(0xffffffffu, z[r], (lane & ~3) + c / CG);
-            z1024[r] = (0x6400u + zr) * 0x10001u;
+            z1024[r] = (0x6400u + z_st[8 * r * GPS + c / CG]) * 0x10001u;
             z64[r] = h2_sub(0x63806380u, z1024[r]);  // 960 - (1024 + z)
           } else {
             z1024[r] = 0x64086408u;  // 1032
@@ -211,8 +232,7 @@ __global__ void __launch_bounds__(W4Cfg<NT>::THREADS, 1)
       if ((c + 1) % CG == 0) {
 #pragma unroll
         for (int r = 0; r < 2 * MT; ++r) {
-          const uint32_t sr = GP == 1 ? sc[r] : __shfl_sync(0xffffffffu, sc[r], (lane & ~3) + c / CG);
-          const float f = __half2float(__ushort_as_half(uint16_t(sr)));
+          const float f = __half2float(sc_st[8 * r * GPS + c / CG]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float* dst = acc[r >> 1][nt] + 2 * (r & 1);
@@ -222,11 +242,6 @@ __global__ void __launch_bounds__(W4Cfg<NT>::THREADS, 1)
           }
         }
       }
-    }
-#pragma unroll
-    for (int r = 0; r < 2 * MT; ++r) {
-      sc[r] = sc1[r];
-      if constexpr (ZEROS) z[r] = z1[r];
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(empty + st);
@@ -239,6 +254,7 @@ __global__ void __launch_bounds__(W4Cfg<NT>::THREADS, 1)
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) acc[mt][nt][0] = acc[mt][nt][1] = acc[mt][nt][2] = acc[mt][nt][3] = __uint_as_float(0x7fc00000u);
+  cp_async_wait_all();
   // a CTA whose wait ran out still has copies on their way into the ring: wait for them (again with a limit)
   if (!__syncthreads_and(ok)) {
     if (tid == 0)
@@ -286,7 +302,7 @@ __global__ void __launch_bounds__(W4Cfg<NT>::THREADS, 1)
 // room, and read from L1 or L2 otherwise.
 struct W4RowsPlan {
   int wm, wk, stages, parts, per;  // parts: CTAs of a cluster that share the columns, `per` stages each
-  int ring;                        // bytes
+  int ring;                        // bytes of the stages with their scales
 };
 constexpr int kW4RowsWarps = 16;
 constexpr int kW4RowsSmem = 224 * 1024, kW4RowsHead = 1024;  // barriers, alignment
@@ -305,44 +321,46 @@ template <int PART, int GROUP, bool ZEROS, bool XS>
 __global__ void __launch_bounds__(32 * kW4RowsWarps, 1)
     w4_rows_kernel(const W4Args a, const W4RowsPlan p, const __grid_constant__ CUtensorMap wmap) {
   constexpr int SUBS = PART / 128, CG = GROUP / 32, SG = 128 / GROUP;  // runs of 128 columns, chunks of a group, groups of a run
-  constexpr int PG = PART / GROUP;                                     // groups of a part:
-  constexpr bool EACH = PG <= 2;                                       // every lane reads its rows' or, with more, one in four
-  constexpr int LG = EACH ? PG : PG / 4;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   __shared__ uint64_t full[32], empty[32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint32_t rank;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-  const int rows = 16 * p.wm, kc = PART * p.wk, stage_bytes = rows * kc / 2;
+  const int rows = 16 * p.wm, kc = PART * p.wk, stage_bytes = rows * kc / 2, gps = kc / GROUP;
+  const int sc_bytes = rows * gps * (ZEROS ? 3 : 2);  // of a stage: [rows][gps] fp16, [rows][gps] bytes
+  uint8_t* scales = smem + p.stages * stage_bytes;
   const int n0 = blockIdx.x / p.parts * rows;
   const int all = (a.K + kc - 1) / kc;
   const int s0 = min(all, int(rank) * p.per), n_st = min(all, s0 + p.per) - s0;
   if (tid < p.stages) {
-    mbar_init(full + tid, 1);
+    mbar_init(full + tid, 1 + rows);
     mbar_init(empty + tid, p.wm * p.wk);
   }
   fence_mbar_init();
   __syncthreads();
-  int filled = 0;  // thread 0: stages whose copies have started
+  // the first `rows` threads start a stage's copies: thread 0 the codes, each its row's scales
+  const int groups = a.K / GROUP;
+  int filled = 0;
   auto fill = [&](int st) {
-    const uint32_t dst = smem_u32(smem + st * stage_bytes);
-    mbar_arrive_expect_tx(full + st, stage_bytes);
-    for (int j = 0; j < kc / 256; ++j)
-      load_2d(dst + j * rows * 128, &wmap, (s0 + filled) * (kc / 2) + j * 128, n0, full + st);
+    if (tid == 0) {
+      const uint32_t dst = smem_u32(smem + st * stage_bytes);
+      mbar_arrive_expect_tx(full + st, stage_bytes);
+      for (int j = 0; j < kc / 256; ++j)
+        load_2d(dst + j * rows * 128, &wmap, (s0 + filled) * (kc / 2) + j * 128, n0, full + st);
+    }
+    uint8_t* sc = scales + st * sc_bytes;
+    copy_scales<ZEROS>(a, sc + tid * gps * 2, sc + rows * gps * 2 + tid * gps, min(n0 + tid, a.N - 1), groups, (s0 + filled) * gps,
+                       gps, full + st);
     ++filled;
   };
-  if (tid == 0)
+  if (tid < rows)
     while (filled < min(p.stages, n_st)) fill(filled);
 
   const int wm = warp % p.wm, wk = warp / p.wm;
-  const int groups = a.K / GROUP;
-  uint32_t at[2];  // scale rows (behind N: the last one's, not stored)
-#pragma unroll
-  for (int r = 0; r < 2; ++r) at[r] = min(n0 + wm * 16 + g + 8 * r, a.N - 1) * uint32_t(groups);
   const int xr = min((g & 1) * 4 + (g >> 1), a.B - 1);  // the batch row that is column g (as above); behind the batch: the last, not stored
   const uint32_t pitch = p.per * kc * 2 + 16;           // of a row of x in shared memory: rows r and r + 4 half the banks apart
-  uint8_t* xsm = smem + p.ring;
+  uint8_t* xsm = smem + p.ring;  // (behind the scales)
   if constexpr (XS) {
     const int cols = n_st * kc / 8;
     for (int b = 0; b < a.B; ++b)
@@ -370,20 +388,9 @@ __global__ void __launch_bounds__(32 * kW4RowsWarps, 1)
   const uint8_t* x_lane = xsm + xr * pitch + wk * PART * 2 + 16 * t;
   const __half* xrow = a.x + (size_t)xr * a.K + 8 * t;
   uint4 xs[XS ? 1 : 4];
-  uint32_t sc[2][LG], z[2][LG];
-  auto fetch_scales = [&](int k, uint32_t (&sc)[2][LG], uint32_t (&z)[2][LG]) {
-#pragma unroll
-    for (int j = 0; j < LG; ++j) {
-      const int gr = k / GROUP + (EACH ? j : 4 * j + t);
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        sc[r][j] = gr < groups ? __half_as_ushort(a.scales[at[r] + gr]) : 0u;
-        if constexpr (ZEROS) z[r][j] = gr < groups ? a.zeros[at[r] + gr] : 8u;
-      }
-    }
-  };
+  // this lane's weight rows of the CTA's are 16 wm + g + 8 r (behind N: the last one's scales, not stored)
+  const int sc_at = (wm * 16 + g) * gps + wk * (PART / GROUP);
   int k = s0 * kc + wk * PART;  // this warp's first column of the stage
-  fetch_scales(k, sc, z);
   if constexpr (!XS) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) xs[c] = k + 32 * c < a.K ? *reinterpret_cast<const uint4*>(xrow + k + 32 * c) : make_uint4(0u, 0u, 0u, 0u);
@@ -395,21 +402,16 @@ __global__ void __launch_bounds__(32 * kW4RowsWarps, 1)
   float acc[4] = {};
 #pragma unroll 1
   for (int i = 0; i < n_st; ++i) {
-    uint32_t sc1[2][LG], z1[2][LG];
-    if (i + 4 < n_st && lane < 16) {  // the scales of four stages on, into L2
-      const uint32_t far = min(n0 + wm * 16 + lane, a.N - 1) * uint32_t(groups) + min((k + 4 * kc) / GROUP, groups - 1);
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(a.scales + far));
-      if constexpr (ZEROS) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.zeros + far));
-    }
-    fetch_scales(k + kc, sc1, z1);
     ok = __all_sync(0xffffffffu, ok && wait(full + st, parity));
     if (!ok) break;
-    if (tid == 0 && i > 0 && filled < n_st) {  // the stage before this one, once all warps have left it
+    if (tid < rows && i > 0 && filled < n_st) {  // the stage before this one, once all warps have left it
       const int before = st == 0 ? p.stages - 1 : st - 1;
       ok = wait(empty + before, st == 0 ? parity ^ 1 : parity);
       if (ok) fill(before);
     }
     const uint32_t w_st = smem_u32(smem) + st * stage_bytes + w_lane;
+    const __half* sc_st = reinterpret_cast<const __half*>(scales + st * sc_bytes) + sc_at;
+    const uint8_t* z_st = scales + st * sc_bytes + rows * gps * 2 + sc_at;
 #pragma unroll
     for (int sub = 0; sub < SUBS; ++sub) {
       const uint32_t w_at = PART == 128 ? w_st : (w_st + (sub >> 1) * rows * 128) ^ ((sub & 1) << 6);
@@ -422,8 +424,7 @@ __global__ void __launch_bounds__(32 * kW4RowsWarps, 1)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             if constexpr (ZEROS) {
-              const uint32_t zr = EACH ? z[r][j % LG] : __shfl_sync(0xffffffffu, z[r][(j / 4) % LG], (lane & ~3) + j % 4);
-              z1024[r] = (0x6400u + zr) * 0x10001u;
+              z1024[r] = (0x6400u + z_st[8 * r * gps + j]) * 0x10001u;
               z64[r] = h2_sub(0x63806380u, z1024[r]);  // 960 - (1024 + z)
             } else {
               z1024[r] = 0x64086408u;  // 1032
@@ -457,8 +458,7 @@ __global__ void __launch_bounds__(32 * kW4RowsWarps, 1)
         if ((c + 1) % CG == 0) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const uint32_t sr = EACH ? sc[r][j % LG] : __shfl_sync(0xffffffffu, sc[r][(j / 4) % LG], (lane & ~3) + j % 4);
-            const float f = __half2float(__ushort_as_half(uint16_t(sr)));
+            const float f = __half2float(sc_st[8 * r * gps + j]);
             acc[2 * r] += f * (d[2 * r] + e[2 * r]);
             acc[2 * r + 1] += f * (d[2 * r + 1] + e[2 * r + 1]);
           }
@@ -467,18 +467,12 @@ __global__ void __launch_bounds__(32 * kW4RowsWarps, 1)
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(empty + st);
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-      for (int j = 0; j < LG; ++j) {
-        sc[r][j] = sc1[r][j];
-        if constexpr (ZEROS) z[r][j] = z1[r][j];
-      }
     k += kc;
     x_lane += 2 * kc;
     st = st + 1 == p.stages ? 0 : st + 1;
     parity ^= st == 0 ? 1u : 0u;
   }
+  cp_async_wait_all();
   // after a wait that ran out: outputs are NaN, and no copy may be on its way when the CTA goes on (waits have a limit)
   if (!__syncthreads_and(ok)) {
     acc[0] = acc[1] = acc[2] = acc[3] = __uint_as_float(0x7fc00000u);
@@ -575,7 +569,7 @@ cudaError_t launch_rows(const W4Args& a, int sms, cudaStream_t s) {
   p.per = (all + p.parts - 1) / p.parts;
   const int64_t x_bytes = (int64_t)a.B * ((int64_t)p.per * PART * p.wk * 2 + 16);
   const bool xs = PART > 128 && x_bytes <= kW4RowsX;
-  const int stage = 16 * p.wm * PART * p.wk / 2;
+  const int stage = 16 * p.wm * PART * p.wk / 2 + 16 * p.wm * (PART * p.wk / GROUP) * (ZEROS ? 3 : 2);
   p.stages = int(std::min<int64_t>(32, (kW4RowsSmem - kW4RowsHead - (xs ? x_bytes : 0)) / stage));
   p.ring = p.stages * stage;
   return xs ? launch_rows_x<PART, GROUP, ZEROS, true>(a, p, ctas, s) : launch_rows_x<PART, GROUP, ZEROS, false>(a, p, ctas, s);
