@@ -15,7 +15,7 @@
 namespace mmc {
 namespace {
 
-constexpr int kAppendThreads = 128;
+constexpr int kAppendThreads = 256;
 constexpr int kAttnWarps = 4;  // warp w reads block w of each page
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -42,11 +42,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-__device__ __forceinline__ uint8_t to_e4m3(float x) {
+__device__ __forceinline__ uint16_t to_e4m3x2(float lo, float hi) {
   uint16_t d;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(0.f), "f"(x));
-  return uint8_t(d);
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
+  return d;
 }
+__device__ __forceinline__ uint8_t to_e4m3(float x) { return uint8_t(to_e4m3x2(x, 0.f)); }
 // two e4m3 codes (low byte first) to fp16: exact
 __device__ __forceinline__ uint32_t e4m3x2_half2(uint32_t two) {
   uint32_t d;
@@ -60,159 +61,213 @@ __device__ __forceinline__ float from_e4m3(uint8_t c) {
 
 // ---------------------------------------------------------------- append
 
-// One CTA per row. Its warps take the row's q heads (RMSNorm, rotation, fp16),
-// and where the row is the first of this call in its block of 16 positions, the
-// block's K and V of each kv head: one warp holds the block's new rows in
-// registers, finds their largest magnitude, takes the older codes over to the
-// new scale if it grew, and writes the new codes. A block has one owner, so no
-// atomics and no order that could change the result.
-template <int HD>
-__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8AppendArgs a) {
-  constexpr int HALF = HD / 2;
-  constexpr int PP = (HALF + 31) / 32;  // (d, d + HALF) pairs of a lane
-  const Kv8Args& c = a.c;
-  const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  __shared__ int s_seq, s_twice;
-  if (tid == 0) {
-    s_seq = -1;
-    s_twice = 0;
-  }
-  __syncthreads();
-  if (c.row_start == nullptr) {
-    if (tid == 0) s_seq = row < c.n_seqs ? row : -1;
-  } else {
-    for (int i = tid; i < c.n_seqs; i += kAppendThreads)
-      if (c.row_start[i] <= row && row < c.row_start[i + 1]) s_seq = i;
-  }
-  __syncthreads();
-  const int seq = s_seq;
-  if (seq < 0) return;  // a row behind the last sequence
-  const int slot = c.slots[seq];
-  if (slot < 0) return;  // an unused sequence
-  const int first = c.row_start ? c.row_start[seq] : seq;
-  const int last = c.row_start ? c.row_start[seq + 1] : seq + 1;
-  if (slot >= c.max_seqs) {
-    if (tid == 0) set_error(c.err, kDevBadSlot);
-    return;
-  }
-  if (first < 0 || last > c.rows || last - first > c.max_new) {
-    if (tid == 0) set_error(c.err, kDevBadRows);
-    return;
-  }
-  for (int i = tid; i < c.n_seqs; i += kAppendThreads)
-    if (i != seq && c.slots[i] == slot && (c.row_start == nullptr || c.row_start[i] < c.row_start[i + 1])) s_twice = 1;
-  __syncthreads();
-  if (s_twice) {
-    if (tid == 0) set_error(c.err, kDevSlotTwice);
-    return;
-  }
-  const int pos0 = c.seq_pos[slot];
-  if (pos0 < 0 || (int64_t)pos0 + (last - first) > (int64_t)c.max_pages * kPageTokens) {
-    if (tid == 0) set_error(c.err, kDevContextLimit);
-    return;
-  }
-  if (pos0 + (last - first) > a.max_pos) {
-    if (tid == 0) set_error(c.err, kDevPositionLimit);
-    return;
-  }
-  const int pos = pos0 + (row - first);
-  const int heads = c.nq + 2 * c.nkv;
+// One CTA per window of `window` rows. A head's row is held by hd / 8 lanes, four
+// elements of each half a lane, so that a lane has both ends of its rotations and
+// loads and stores are 16, 8 (fp16 q) and 4 (codes) bytes wide; a warp takes as
+// many rows of a head as fit. Units of work, dealt to the warps: the window's q
+// heads (RMSNorm, rotation, fp16), and for each row that is the first of this
+// call in its block of 16 positions, the block's K or V of one kv head: the warp
+// holds the block's new rows in registers, finds their largest magnitude, takes
+// the older codes over to the new scale if it grew, and writes the new codes. A
+// block has one owner, so no atomics and no order that could change the result.
+//   Bound by HBM with many rows (the raw projections are four times the bytes of
+// all that is written); with few, by the chain of loads slot -> position -> page
+// -> old scale, so the projections are loaded before it.
+constexpr int kMaxWindow = 16;
 
-  // norm and rotation of one head of row r at position p: x[i][0] is element lane + 32 i, x[i][1] its partner
-  auto turned = [&](int r, int head, const float* w, int p, float (&x)[PP][2]) {
-    const float* src = a.qkv + ((size_t)r * heads + head) * HD;
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < PP; ++i) {
-      const int d = lane + 32 * i;
-      x[i][0] = d < HALF ? src[d] : 0.f;
-      x[i][1] = d < HALF ? src[d + HALF] : 0.f;
-      ss += x[i][0] * x[i][0] + x[i][1] * x[i][1];
+template <int HD>
+__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8AppendArgs a, int window) {
+  constexpr int HALF = HD / 2, LPH = HD / 8;                                    // lanes of a head's row
+  constexpr int GL = LPH <= 2 ? 2 : LPH <= 4 ? 4 : LPH <= 8 ? 8 : 16;           // lanes of a group
+  constexpr int HPW = 32 / GL, ITS = (kKv8Block + HPW - 1) / HPW, BATCH = 4;
+  constexpr int WARPS = kAppendThreads / 32;
+  const Kv8Args& c = a.c;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane / GL, gl = lane % GL;
+  const bool in = gl < LPH;
+  const int d0 = 4 * (in ? gl : 0);
+  const int row0 = blockIdx.x * window, nrows = min(window, c.rows - row0);
+  const int heads = c.nq + 2 * c.nkv;
+  __shared__ int s_seq[kMaxWindow], s_slot[kMaxWindow], s_first[kMaxWindow], s_last[kMaxWindow], s_twice[kMaxWindow];
+  __shared__ int s_pos[kMaxWindow];   // position, -1: not of any sequence, unused or refused
+  __shared__ int s_lead[kMaxWindow];  // rows that own a block
+  __shared__ int s_leads;
+
+  struct Row8 {
+    float4 lo, hi;  // elements d0 .. + 3 of the first and of the second half
+  };
+  auto load = [&](int row, int head) {
+    Row8 x{make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+    if (in) {
+      const float* src = a.qkv + ((size_t)row * heads + head) * HD + d0;
+      x.lo = *reinterpret_cast<const float4*>(src);
+      x.hi = *reinterpret_cast<const float4*>(src + HALF);
     }
-    float rs = 1.f;
-    if (w != nullptr) rs = 1.0f / sqrtf(warp_sum(ss) / float(HD) + a.eps);
+    return x;
+  };
+  // the q units of a window: (row, HPW heads); the first batch is loaded ahead of everything else
+  const int per_row = (c.nq + HPW - 1) / HPW, q_units = nrows * per_row;
+  Row8 x[BATCH];
+  auto load_batch = [&](int u0) {
 #pragma unroll
-    for (int i = 0; i < PP; ++i) {
-      const int d = lane + 32 * i;
-      if (d >= HALF) continue;
-      const float u = w ? x[i][0] * rs * w[d] : x[i][0], v = w ? x[i][1] * rs * w[d + HALF] : x[i][1];
-      const float co = a.rope_cos[(size_t)p * HALF + d], si = a.rope_sin[(size_t)p * HALF + d];
-      x[i][0] = u * co - v * si;
-      x[i][1] = v * co + u * si;
+    for (int b = 0; b < BATCH; ++b) {
+      const int u = u0 + b * WARPS;
+      if (u < q_units) x[b] = load(row0 + u / per_row, min(u % per_row * HPW + grp, c.nq - 1));
     }
   };
+  load_batch(warp);
 
-  for (int h = warp; h < c.nq; h += kAppendThreads / 32) {
-    float x[PP][2];
-    turned(row, h, a.q_norm, pos, x);
-    __half* dst = a.q + ((size_t)row * c.nq + h) * HD;
+  // ---- which sequence each row of the window belongs to, and whether its slot appears twice
+  if (tid < window) {
+    s_seq[tid] = -1;
+    s_slot[tid] = -1;
+    s_twice[tid] = 0;
+  }
+  if (tid == 0) s_leads = 0;
+  __syncthreads();
+  int my_slot = -1;  // of sequence tid (the first round of the loop)
+  bool my_rows = false;
+  for (int i = tid; i < c.n_seqs; i += kAppendThreads) {
+    const int b = c.row_start ? c.row_start[i] : i, e = c.row_start ? c.row_start[i + 1] : i + 1, slot = c.slots[i];
+    if (i == tid) {
+      my_slot = slot;
+      my_rows = b < e;
+    }
+    for (int r = max(b, row0); r < min(e, row0 + nrows); ++r) {
+      s_seq[r - row0] = i;
+      s_slot[r - row0] = slot;
+      s_first[r - row0] = b;
+      s_last[r - row0] = e;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < c.n_seqs; i += kAppendThreads) {
+    const int slot = i == tid ? my_slot : c.slots[i];
+    if (slot < 0) continue;
+    for (int r = 0; r < nrows; ++r)
+      if (s_slot[r] == slot && s_seq[r] != i && (i == tid ? my_rows : c.row_start == nullptr || c.row_start[i] < c.row_start[i + 1]))
+        s_twice[r] = 1;
+  }
+  int pos0 = 0;
+  const int slot = tid < nrows ? s_slot[tid] : -1;
+  if (slot >= 0 && slot < c.max_seqs) pos0 = c.seq_pos[slot];
+  __syncthreads();
+  if (tid < nrows) {
+    int pos = -1, e = 0;
+    if (s_seq[tid] >= 0 && slot >= 0) {
+      const int first = s_first[tid], last = s_last[tid];
+      if (slot >= c.max_seqs) e = kDevBadSlot;
+      else if (first < 0 || last > c.rows || last - first > c.max_new) e = kDevBadRows;
+      else if (s_twice[tid]) e = kDevSlotTwice;
+      else if (pos0 < 0 || (int64_t)pos0 + (last - first) > (int64_t)c.max_pages * kPageTokens) e = kDevContextLimit;
+      else if (pos0 + (last - first) > a.max_pos) e = kDevPositionLimit;
+      else pos = pos0 + (row0 + tid - first);
+      if (e != 0) set_error(c.err, e);
+    }
+    s_pos[tid] = pos;
+    // the first row of this call in its block writes the block
+    if (pos >= 0 && (row0 + tid == s_first[tid] || pos % kKv8Block == 0)) s_lead[atomicAdd(&s_leads, 1)] = tid;
+  }
+  __syncthreads();
+
+  // norm (w != null) and rotation of a row at position p
+  auto norm = [&](Row8& v, const float* w) {
+    if (w == nullptr) return;
+    float ss = v.lo.x * v.lo.x + v.lo.y * v.lo.y + v.lo.z * v.lo.z + v.lo.w * v.lo.w + v.hi.x * v.hi.x + v.hi.y * v.hi.y +
+               v.hi.z * v.hi.z + v.hi.w * v.hi.w;
 #pragma unroll
-    for (int i = 0; i < PP; ++i) {
-      const int d = lane + 32 * i;
-      if (d < HALF) {
-        dst[d] = __float2half_rn(x[i][0]);
-        dst[d + HALF] = __float2half_rn(x[i][1]);
+    for (int o = GL / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float rs = 1.0f / sqrtf(ss / float(HD) + a.eps);
+    const float4 wl = *reinterpret_cast<const float4*>(w + d0), wh = *reinterpret_cast<const float4*>(w + d0 + HALF);
+    v.lo = make_float4(v.lo.x * rs * wl.x, v.lo.y * rs * wl.y, v.lo.z * rs * wl.z, v.lo.w * rs * wl.w);
+    v.hi = make_float4(v.hi.x * rs * wh.x, v.hi.y * rs * wh.y, v.hi.z * rs * wh.z, v.hi.w * rs * wh.w);
+  };
+  auto turn = [&](Row8& v, int p) {
+    const float4 co = *reinterpret_cast<const float4*>(a.rope_cos + (size_t)p * HALF + d0);
+    const float4 si = *reinterpret_cast<const float4*>(a.rope_sin + (size_t)p * HALF + d0);
+    const Row8 u = v;
+    v.lo = make_float4(u.lo.x * co.x - u.hi.x * si.x, u.lo.y * co.y - u.hi.y * si.y, u.lo.z * co.z - u.hi.z * si.z,
+                       u.lo.w * co.w - u.hi.w * si.w);
+    v.hi = make_float4(u.hi.x * co.x + u.lo.x * si.x, u.hi.y * co.y + u.lo.y * si.y, u.hi.z * co.z + u.lo.z * si.z,
+                       u.hi.w * co.w + u.lo.w * si.w);
+  };
+
+  for (int u0 = warp; u0 < q_units; u0 += BATCH * WARPS) {
+    if (u0 != warp) load_batch(u0);
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      const int u = u0 + b * WARPS;
+      if (u >= q_units) break;
+      const int r = u / per_row, h = u % per_row * HPW + grp, pos = s_pos[r];
+      if (pos < 0) continue;  // (uniform in the warp)
+      norm(x[b], a.q_norm);
+      turn(x[b], pos);
+      if (in && h < c.nq) {
+        __half* dst = a.q + ((size_t)(row0 + r) * c.nq + h) * HD + d0;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_half2(x[b].lo.x, x[b].lo.y), pack_half2(x[b].lo.z, x[b].lo.w));
+        *reinterpret_cast<uint2*>(dst + HALF) = make_uint2(pack_half2(x[b].hi.x, x[b].hi.y), pack_half2(x[b].hi.z, x[b].hi.w));
       }
     }
   }
 
-  // the first row of this call in its block writes the block
-  if (row != first && pos % kKv8Block != 0) return;
-  const int page = c.table[(size_t)slot * c.max_pages + pos / kPageTokens];
-  if (page < 0 || page >= c.n_pages) {
-    if (tid == 0) set_error(c.err, kDevNoPage);
-    return;
-  }
-  const int r0 = pos % kPageTokens, blk = r0 / kKv8Block, older = pos % kKv8Block;
-  const int n = min(kKv8Block - older, last - row);
-  for (int u = warp; u < 2 * c.nkv; u += kAppendThreads / 32) {
-    const int kv = u / c.nkv, h = u % c.nkv;
+  const int leads = s_leads;
+  for (int u = warp; u < leads * 2 * c.nkv; u += WARPS) {
+    const int lead = s_lead[u / (2 * c.nkv)], kv = u % (2 * c.nkv) / c.nkv, h = u % c.nkv;
+    const int row = row0 + lead, pos = s_pos[lead];
+    const int r0 = pos % kPageTokens, blk = r0 / kKv8Block, older = row == s_first[lead] ? pos % kKv8Block : 0;
+    const int n = min(kKv8Block - older, s_last[lead] - row);
+    const int page = c.table[(size_t)s_slot[lead] * c.max_pages + pos / kPageTokens];
+    Row8 v[ITS];
+#pragma unroll
+    for (int i = 0; i < ITS; ++i)
+      if (i * HPW < n) v[i] = load(row + min(i * HPW + grp, n - 1), c.nq + kv * c.nkv + h);
+    if (page < 0 || page >= c.n_pages) {
+      if (lane == 0) set_error(c.err, kDevNoPage);
+      continue;
+    }
     const size_t slab = kv8_slab(c, page, kv, h);
     uint8_t* codes = c.codes + slab * (kPageTokens * HD);
     float* scale = c.scales + slab * kKv8BlocksPerPage + blk;
-    float x[kKv8Block][PP][2];
+    const float had = older > 0 ? *scale : 0.f;
     float amax = 0.f;
 #pragma unroll
-    for (int j = 0; j < kKv8Block; ++j) {
-      if (j >= n) break;
+    for (int i = 0; i < ITS; ++i) {
+      if (i * HPW >= n) break;
       if (kv == 0) {
-        turned(row + j, c.nq + h, a.k_norm, pos + j, x[j]);
-      } else {
-        const float* src = a.qkv + ((size_t)(row + j) * heads + c.nq + c.nkv + h) * HD;
-#pragma unroll
-        for (int i = 0; i < PP; ++i) {
-          const int d = lane + 32 * i;
-          x[j][i][0] = d < HALF ? src[d] : 0.f;
-          x[j][i][1] = d < HALF ? src[d + HALF] : 0.f;
-        }
+        norm(v[i], a.k_norm);
+        turn(v[i], pos + min(i * HPW + grp, n - 1));
       }
-#pragma unroll
-      for (int i = 0; i < PP; ++i) amax = max_nan(amax, max_nan(fabsf(x[j][i][0]), fabsf(x[j][i][1])));
+      if (in) {
+        const float lo = max_nan(max_nan(fabsf(v[i].lo.x), fabsf(v[i].lo.y)), max_nan(fabsf(v[i].lo.z), fabsf(v[i].lo.w)));
+        const float hi = max_nan(max_nan(fabsf(v[i].hi.x), fabsf(v[i].hi.y)), max_nan(fabsf(v[i].hi.z), fabsf(v[i].hi.w)));
+        amax = max_nan(amax, max_nan(lo, hi));
+      }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     float s = pow2_scale(amax);
-    const float had = older > 0 ? *scale : 0.f;
     if (older > 0) s = max_nan(s, had);
     if (older > 0 && s > had) {  // (false where s is NaN: a block that is lost keeps its codes)
-      for (int e = lane; e < older * HD; e += 32) {
-        uint8_t* p = codes + (size_t)(blk * kKv8Block) * HD + e;
-        *p = to_e4m3(from_e4m3(*p) * (had / s));
+      for (int e = lane; e < older * HD / 4; e += 32) {
+        uint32_t* p = reinterpret_cast<uint32_t*>(codes + (size_t)(blk * kKv8Block) * HD) + e;
+        const uint32_t was = *p;
+        uint32_t now = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) now |= uint32_t(to_e4m3(from_e4m3(uint8_t(was >> 8 * b)) * (had / s))) << 8 * b;
+        *p = now;
       }
     }
     const bool lost = s != s;
     const float inv = lost ? 0.f : pow2_inverse(s);
+    auto four = [&](const float4& f) {
+      return lost ? 0u : uint32_t(to_e4m3x2(f.x * inv, f.y * inv)) | uint32_t(to_e4m3x2(f.z * inv, f.w * inv)) << 16;
+    };
 #pragma unroll
-    for (int j = 0; j < kKv8Block; ++j) {
-      if (j >= n) break;
-      uint8_t* dst = codes + (size_t)(r0 + j) * HD;
-#pragma unroll
-      for (int i = 0; i < PP; ++i) {
-        const int d = lane + 32 * i;
-        if (d < HALF) {
-          dst[d] = lost ? 0 : to_e4m3(x[j][i][0] * inv);
-          dst[d + HALF] = lost ? 0 : to_e4m3(x[j][i][1] * inv);
-        }
+    for (int i = 0; i < ITS; ++i) {
+      const int j = i * HPW + grp;
+      if (j < n && in) {
+        uint8_t* dst = codes + (size_t)(r0 + j) * HD + d0;
+        *reinterpret_cast<uint32_t*>(dst) = four(v[i].lo);
+        *reinterpret_cast<uint32_t*>(dst + HALF) = four(v[i].hi);
       }
     }
     __syncwarp();
@@ -729,7 +784,8 @@ cudaError_t attention_hd(const Kv8AttnArgs& a, cudaStream_t s) {
 
 template <int HD>
 cudaError_t append_hd(const Kv8AppendArgs& a, cudaStream_t s) {
-  kv8_append_kernel<HD><<<a.c.rows, kAppendThreads, 0, s>>>(a);
+  const int window = a.c.max_new == 1 ? 1 : a.c.max_new <= 4 ? 4 : kMaxWindow;  // about one block of a sequence
+  kv8_append_kernel<HD><<<(a.c.rows + window - 1) / window, kAppendThreads, 0, s>>>(a, window);
   return cudaGetLastError();
 }
 
