@@ -63,23 +63,26 @@ __device__ __forceinline__ float from_e4m3(uint8_t c) {
 
 // One CTA per window of `window` rows. A head's row is held by hd / 8 lanes, four
 // elements of each half a lane, so that a lane has both ends of its rotations and
-// loads and stores are 16, 8 (fp16 q) and 4 (codes) bytes wide; a warp takes as
-// many rows of a head as fit. Units of work, dealt to the warps: the window's q
-// heads (RMSNorm, rotation, fp16), and for each row that is the first of this
-// call in its block of 16 positions, the block's K or V of one kv head: the warp
-// holds the block's new rows in registers, finds their largest magnitude, takes
-// the older codes over to the new scale if it grew, and writes the new codes. A
-// block has one owner, so no atomics and no order that could change the result.
+// loads and stores are 16, 8 (fp16 q) and 4 (codes) bytes wide. The q heads
+// (RMSNorm, rotation, fp16) are dealt to the warps. Then, for each row that is the
+// first of this call in its block of 16 positions, the CTA takes the whole block,
+// four of its K and V heads at a time: the new rows stay in registers while their
+// largest magnitudes go through shared memory, older codes go over to the new
+// scale if it grew, and the new codes are written. With at most kStepRows rows a
+// sequence (STEP) a window is one row and each K or V head one warp's, without
+// barriers. A block has one owner, so no atomics on the cache and no order that
+// could change the result.
 //   Bound by HBM with many rows (the raw projections are four times the bytes of
 // all that is written); with few, by the chain of loads slot -> position -> page
 // -> old scale, so the projections are loaded before it.
-constexpr int kMaxWindow = 16;
+constexpr int kWindow = 8, kStepRows = 8;
 
-template <int HD>
-__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8AppendArgs a, int window) {
+template <int HD, bool STEP>
+__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8AppendArgs a) {
+  constexpr int window = STEP ? 1 : kWindow;
   constexpr int HALF = HD / 2, LPH = HD / 8;                                    // lanes of a head's row
   constexpr int GL = LPH <= 2 ? 2 : LPH <= 4 ? 4 : LPH <= 8 ? 8 : 16;           // lanes of a group
-  constexpr int HPW = 32 / GL, ITS = (kKv8Block + HPW - 1) / HPW, BATCH = 4;
+  constexpr int HPW = 32 / GL, BATCH = STEP ? 1 : 4;                                    // heads of a warp at once, and of a unit
   constexpr int WARPS = kAppendThreads / 32;
   const Kv8Args& c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane / GL, gl = lane % GL;
@@ -87,9 +90,9 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8App
   const int d0 = 4 * (in ? gl : 0);
   const int row0 = blockIdx.x * window, nrows = min(window, c.rows - row0);
   const int heads = c.nq + 2 * c.nkv;
-  __shared__ int s_seq[kMaxWindow], s_slot[kMaxWindow], s_first[kMaxWindow], s_last[kMaxWindow], s_twice[kMaxWindow];
-  __shared__ int s_pos[kMaxWindow];   // position, -1: not of any sequence, unused or refused
-  __shared__ int s_lead[kMaxWindow];  // rows that own a block
+  __shared__ int s_seq[kWindow], s_slot[kWindow], s_first[kWindow], s_last[kWindow], s_twice[kWindow];
+  __shared__ int s_pos[kWindow];   // position, -1: not of any sequence, unused or refused
+  __shared__ int s_lead[kWindow];  // rows that own a block
   __shared__ int s_leads;
 
   struct Row8 {
@@ -104,17 +107,22 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8App
     }
     return x;
   };
-  // the q units of a window: (row, HPW heads); the first batch is loaded ahead of everything else
-  const int per_row = (c.nq + HPW - 1) / HPW, q_units = nrows * per_row;
+  // the q units of a window: BATCH * HPW heads of a row; the first is loaded ahead of everything else
+  const int per_row = (c.nq + BATCH * HPW - 1) / (BATCH * HPW), q_units = nrows * per_row;
   Row8 x[BATCH];
-  auto load_batch = [&](int u0) {
+  auto load_unit = [&](int u) {
 #pragma unroll
-    for (int b = 0; b < BATCH; ++b) {
-      const int u = u0 + b * WARPS;
-      if (u < q_units) x[b] = load(row0 + u / per_row, min(u % per_row * HPW + grp, c.nq - 1));
-    }
+    for (int b = 0; b < BATCH; ++b)
+      x[b] = load(row0 + u / per_row, min((u % per_row * BATCH + b) * HPW + grp, c.nq - 1));
   };
-  load_batch(warp);
+  if (warp < q_units) load_unit(warp);
+  // STEP: K and V heads, one a warp, from the last warp on
+  constexpr int ITS = (kStepRows + HPW - 1) / HPW;
+  Row8 v[STEP ? ITS : 1];
+  const int kv_first = WARPS - 1 - warp;
+  if constexpr (STEP) {
+    if (c.max_new == 1 && kv_first < 2 * c.nkv) v[0] = load(row0, c.nq + kv_first);
+  }
 
   // ---- which sequence each row of the window belongs to, and whether its slot appears twice
   if (tid < window) {
@@ -169,109 +177,188 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8App
   }
   __syncthreads();
 
-  // norm (w != null) and rotation of a row at position p
-  auto norm = [&](Row8& v, const float* w) {
-    if (w == nullptr) return;
+  auto weights = [&](const float* w) {  // of a norm
+    Row8 v{};
+    if (w != nullptr) {
+      v.lo = *reinterpret_cast<const float4*>(w + d0);
+      v.hi = *reinterpret_cast<const float4*>(w + d0 + HALF);
+    }
+    return v;
+  };
+  auto angles = [&](int p) {  // cosines, sines
+    return Row8{*reinterpret_cast<const float4*>(a.rope_cos + (size_t)p * HALF + d0),
+                *reinterpret_cast<const float4*>(a.rope_sin + (size_t)p * HALF + d0)};
+  };
+  auto norm = [&](Row8& v, const Row8& w) {
     float ss = v.lo.x * v.lo.x + v.lo.y * v.lo.y + v.lo.z * v.lo.z + v.lo.w * v.lo.w + v.hi.x * v.hi.x + v.hi.y * v.hi.y +
                v.hi.z * v.hi.z + v.hi.w * v.hi.w;
 #pragma unroll
     for (int o = GL / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     const float rs = 1.0f / sqrtf(ss / float(HD) + a.eps);
-    const float4 wl = *reinterpret_cast<const float4*>(w + d0), wh = *reinterpret_cast<const float4*>(w + d0 + HALF);
-    v.lo = make_float4(v.lo.x * rs * wl.x, v.lo.y * rs * wl.y, v.lo.z * rs * wl.z, v.lo.w * rs * wl.w);
-    v.hi = make_float4(v.hi.x * rs * wh.x, v.hi.y * rs * wh.y, v.hi.z * rs * wh.z, v.hi.w * rs * wh.w);
+    v.lo = make_float4(v.lo.x * rs * w.lo.x, v.lo.y * rs * w.lo.y, v.lo.z * rs * w.lo.z, v.lo.w * rs * w.lo.w);
+    v.hi = make_float4(v.hi.x * rs * w.hi.x, v.hi.y * rs * w.hi.y, v.hi.z * rs * w.hi.z, v.hi.w * rs * w.hi.w);
   };
-  auto turn = [&](Row8& v, int p) {
-    const float4 co = *reinterpret_cast<const float4*>(a.rope_cos + (size_t)p * HALF + d0);
-    const float4 si = *reinterpret_cast<const float4*>(a.rope_sin + (size_t)p * HALF + d0);
+  auto turn = [&](Row8& v, const Row8& cs) {
     const Row8 u = v;
-    v.lo = make_float4(u.lo.x * co.x - u.hi.x * si.x, u.lo.y * co.y - u.hi.y * si.y, u.lo.z * co.z - u.hi.z * si.z,
-                       u.lo.w * co.w - u.hi.w * si.w);
-    v.hi = make_float4(u.hi.x * co.x + u.lo.x * si.x, u.hi.y * co.y + u.lo.y * si.y, u.hi.z * co.z + u.lo.z * si.z,
-                       u.hi.w * co.w + u.lo.w * si.w);
+    v.lo = make_float4(u.lo.x * cs.lo.x - u.hi.x * cs.hi.x, u.lo.y * cs.lo.y - u.hi.y * cs.hi.y,
+                       u.lo.z * cs.lo.z - u.hi.z * cs.hi.z, u.lo.w * cs.lo.w - u.hi.w * cs.hi.w);
+    v.hi = make_float4(u.hi.x * cs.lo.x + u.lo.x * cs.hi.x, u.hi.y * cs.lo.y + u.lo.y * cs.hi.y,
+                       u.hi.z * cs.lo.z + u.lo.z * cs.hi.z, u.hi.w * cs.lo.w + u.lo.w * cs.hi.w);
   };
 
-  for (int u0 = warp; u0 < q_units; u0 += BATCH * WARPS) {
-    if (u0 != warp) load_batch(u0);
-#pragma unroll
-    for (int b = 0; b < BATCH; ++b) {
-      const int u = u0 + b * WARPS;
-      if (u >= q_units) break;
-      const int r = u / per_row, h = u % per_row * HPW + grp, pos = s_pos[r];
+  {
+    const Row8 w = weights(a.q_norm);
+    for (int u = warp; u < q_units; u += WARPS) {
+      if (u != warp) load_unit(u);
+      const int r = u / per_row, pos = s_pos[r];
       if (pos < 0) continue;  // (uniform in the warp)
-      norm(x[b], a.q_norm);
-      turn(x[b], pos);
-      if (in && h < c.nq) {
-        __half* dst = a.q + ((size_t)(row0 + r) * c.nq + h) * HD + d0;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_half2(x[b].lo.x, x[b].lo.y), pack_half2(x[b].lo.z, x[b].lo.w));
-        *reinterpret_cast<uint2*>(dst + HALF) = make_uint2(pack_half2(x[b].hi.x, x[b].hi.y), pack_half2(x[b].hi.z, x[b].hi.w));
+      const Row8 cs = angles(pos);
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) {
+        const int h = (u % per_row * BATCH + b) * HPW + grp;
+        if (a.q_norm != nullptr) norm(x[b], w);
+        turn(x[b], cs);
+        if (in && h < c.nq) {
+          __half* dst = a.q + ((size_t)(row0 + r) * c.nq + h) * HD + d0;
+          *reinterpret_cast<uint2*>(dst) = make_uint2(pack_half2(x[b].lo.x, x[b].lo.y), pack_half2(x[b].lo.z, x[b].lo.w));
+          *reinterpret_cast<uint2*>(dst + HALF) =
+              make_uint2(pack_half2(x[b].hi.x, x[b].hi.y), pack_half2(x[b].hi.z, x[b].hi.w));
+        }
       }
     }
   }
 
   const int leads = s_leads;
-  for (int u = warp; u < leads * 2 * c.nkv; u += WARPS) {
-    const int lead = s_lead[u / (2 * c.nkv)], kv = u % (2 * c.nkv) / c.nkv, h = u % c.nkv;
-    const int row = row0 + lead, pos = s_pos[lead];
+  // a block's codes: older ones over to a larger scale, by `threads` threads; four new ones
+  auto regrow = [&](uint8_t* block, int older, float f, int thread, int threads) {
+    for (int e = thread; e < older * HD / 4; e += threads) {
+      uint32_t* p = reinterpret_cast<uint32_t*>(block) + e;
+      const uint32_t was = *p;
+      uint32_t now = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) now |= uint32_t(to_e4m3(from_e4m3(uint8_t(was >> 8 * k)) * f)) << 8 * k;
+      *p = now;
+    }
+  };
+  auto four = [&](const float4& f, float inv) {
+    return uint32_t(to_e4m3x2(f.x * inv, f.y * inv)) | uint32_t(to_e4m3x2(f.z * inv, f.w * inv)) << 16;
+  };
+  auto largest = [&](const Row8& f) {
+    const float lo = max_nan(max_nan(fabsf(f.lo.x), fabsf(f.lo.y)), max_nan(fabsf(f.lo.z), fabsf(f.lo.w)));
+    const float hi = max_nan(max_nan(fabsf(f.hi.x), fabsf(f.hi.y)), max_nan(fabsf(f.hi.z), fabsf(f.hi.w)));
+    return max_nan(lo, hi);
+  };
+  if constexpr (STEP) {
+    if (leads == 0) return;
+    const int pos = s_pos[0], r0 = pos % kPageTokens, blk = r0 / kKv8Block;
+    const int older = row0 == s_first[0] ? pos % kKv8Block : 0, n = min(kKv8Block - older, s_last[0] - row0);
+    const int page = c.table[(size_t)s_slot[0] * c.max_pages + pos / kPageTokens];
+    const Row8 w = weights(a.k_norm);
+    for (int u = kv_first; u < 2 * c.nkv; u += WARPS) {
+      if (c.max_new > 1 || u != kv_first) {
+#pragma unroll
+        for (int i = 0; i < ITS; ++i)
+          if (i * HPW < n) v[i] = load(row0 + min(i * HPW + grp, n - 1), c.nq + u);
+      }
+      if (page < 0 || page >= c.n_pages) {
+        if (lane == 0) set_error(c.err, kDevNoPage);
+        break;
+      }
+      const size_t slab = kv8_slab(c, page, u / c.nkv, u % c.nkv);
+      uint8_t* codes = c.codes + slab * (kPageTokens * HD);
+      float* scale = c.scales + slab * kKv8BlocksPerPage + blk;
+      const float had = older > 0 ? *scale : 0.f;
+      float amax = 0.f;
+#pragma unroll
+      for (int i = 0; i < ITS; ++i) {
+        if (i * HPW >= n) break;
+        if (u < c.nkv) {
+          if (a.k_norm != nullptr) norm(v[i], w);
+          turn(v[i], angles(pos + min(i * HPW + grp, n - 1)));
+        }
+        if (in) amax = max_nan(amax, largest(v[i]));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      float s = pow2_scale(amax);
+      if (older > 0) s = max_nan(s, had);
+      if (older > 0 && s > had)  // (false where s is NaN: a block that is lost keeps its codes)
+        regrow(codes + blk * kKv8Block * HD, older, had / s, lane, 32);
+      const bool lost = s != s;
+      const float inv = lost ? 0.f : pow2_inverse(s);
+#pragma unroll
+      for (int i = 0; i < ITS; ++i) {
+        const int j = i * HPW + grp;
+        if (j < n && in) {
+          uint8_t* dst = codes + (size_t)(r0 + j) * HD + d0;
+          *reinterpret_cast<uint32_t*>(dst) = lost ? 0u : four(v[i].lo, inv);
+          *reinterpret_cast<uint32_t*>(dst + HALF) = lost ? 0u : four(v[i].hi, inv);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) *scale = s;
+    }
+    return;
+  }
+  __shared__ float s_amax[2][BATCH][WARPS];
+  int turns = 0;  // of the two buffers of s_amax
+  for (int li = 0; li < leads; ++li) {
+    const int lead = s_lead[li], row = row0 + lead, pos = s_pos[lead];
     const int r0 = pos % kPageTokens, blk = r0 / kKv8Block, older = row == s_first[lead] ? pos % kKv8Block : 0;
     const int n = min(kKv8Block - older, s_last[lead] - row);
     const int page = c.table[(size_t)s_slot[lead] * c.max_pages + pos / kPageTokens];
-    Row8 v[ITS];
-#pragma unroll
-    for (int i = 0; i < ITS; ++i)
-      if (i * HPW < n) v[i] = load(row + min(i * HPW + grp, n - 1), c.nq + kv * c.nkv + h);
-    if (page < 0 || page >= c.n_pages) {
-      if (lane == 0) set_error(c.err, kDevNoPage);
+    const int j = warp * HPW + grp;  // this group's row of the new ones
+    const bool mine = in && j < n;
+    const Row8 w = weights(a.k_norm), cs = angles(pos + min(j, n - 1));
+    if (page < 0 || page >= c.n_pages) {  // (uniform in the CTA)
+      if (tid == 0) set_error(c.err, kDevNoPage);
       continue;
     }
-    const size_t slab = kv8_slab(c, page, kv, h);
-    uint8_t* codes = c.codes + slab * (kPageTokens * HD);
-    float* scale = c.scales + slab * kKv8BlocksPerPage + blk;
-    const float had = older > 0 ? *scale : 0.f;
-    float amax = 0.f;
+    for (int u0 = 0; u0 < 2 * c.nkv; u0 += BATCH, turns ^= 1) {  // units: K of each kv head, then V
+      Row8 v[BATCH];
+      float had[BATCH];
+      const int m = min(BATCH, 2 * c.nkv - u0);
 #pragma unroll
-    for (int i = 0; i < ITS; ++i) {
-      if (i * HPW >= n) break;
-      if (kv == 0) {
-        norm(v[i], a.k_norm);
-        turn(v[i], pos + min(i * HPW + grp, n - 1));
+      for (int b = 0; b < BATCH; ++b) {
+        const int u = u0 + min(b, m - 1);
+        v[b] = load(row + min(j, n - 1), c.nq + u);
+        had[b] = older > 0 ? c.scales[kv8_slab(c, page, u / c.nkv, u % c.nkv) * kKv8BlocksPerPage + blk] : 0.f;
       }
-      if (in) {
-        const float lo = max_nan(max_nan(fabsf(v[i].lo.x), fabsf(v[i].lo.y)), max_nan(fabsf(v[i].lo.z), fabsf(v[i].lo.w)));
-        const float hi = max_nan(max_nan(fabsf(v[i].hi.x), fabsf(v[i].hi.y)), max_nan(fabsf(v[i].hi.z), fabsf(v[i].hi.w)));
-        amax = max_nan(amax, max_nan(lo, hi));
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) {
+        if (u0 + b < c.nkv) {
+          if (a.k_norm != nullptr) norm(v[b], w);
+          turn(v[b], cs);
+        }
+        float amax = mine ? largest(v[b]) : 0.f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if (lane == 0) s_amax[turns][b][warp] = amax;
+      }
+      __syncthreads();  // (every thread has read the old scales, too)
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) {
+        if (b >= m) break;
+        const int u = u0 + b;
+        const size_t slab = kv8_slab(c, page, u / c.nkv, u % c.nkv);
+        uint8_t* codes = c.codes + slab * (kPageTokens * HD);
+        float amax = 0.f;
+#pragma unroll
+        for (int k = 0; k < WARPS; ++k) amax = max_nan(amax, s_amax[turns][b][k]);
+        float s = pow2_scale(amax);
+        if (older > 0) s = max_nan(s, had[b]);
+        if (older > 0 && s > had[b])  // (false where s is NaN: a block that is lost keeps its codes)
+          regrow(codes + blk * kKv8Block * HD, older, had[b] / s, tid, kAppendThreads);
+        const bool lost = s != s;
+        const float inv = lost ? 0.f : pow2_inverse(s);
+        if (mine) {
+          uint8_t* dst = codes + (size_t)(r0 + j) * HD + d0;
+          *reinterpret_cast<uint32_t*>(dst) = lost ? 0u : four(v[b].lo, inv);
+          *reinterpret_cast<uint32_t*>(dst + HALF) = lost ? 0u : four(v[b].hi, inv);
+        }
+        if (tid == b) c.scales[slab * kKv8BlocksPerPage + blk] = s;
       }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    float s = pow2_scale(amax);
-    if (older > 0) s = max_nan(s, had);
-    if (older > 0 && s > had) {  // (false where s is NaN: a block that is lost keeps its codes)
-      for (int e = lane; e < older * HD / 4; e += 32) {
-        uint32_t* p = reinterpret_cast<uint32_t*>(codes + (size_t)(blk * kKv8Block) * HD) + e;
-        const uint32_t was = *p;
-        uint32_t now = 0;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) now |= uint32_t(to_e4m3(from_e4m3(uint8_t(was >> 8 * b)) * (had / s))) << 8 * b;
-        *p = now;
-      }
-    }
-    const bool lost = s != s;
-    const float inv = lost ? 0.f : pow2_inverse(s);
-    auto four = [&](const float4& f) {
-      return lost ? 0u : uint32_t(to_e4m3x2(f.x * inv, f.y * inv)) | uint32_t(to_e4m3x2(f.z * inv, f.w * inv)) << 16;
-    };
-#pragma unroll
-    for (int i = 0; i < ITS; ++i) {
-      const int j = i * HPW + grp;
-      if (j < n && in) {
-        uint8_t* dst = codes + (size_t)(r0 + j) * HD + d0;
-        *reinterpret_cast<uint32_t*>(dst) = four(v[i].lo);
-        *reinterpret_cast<uint32_t*>(dst + HALF) = four(v[i].hi);
-      }
-    }
-    __syncwarp();
-    if (lane == 0) *scale = s;
   }
 }
 
@@ -784,8 +871,10 @@ cudaError_t attention_hd(const Kv8AttnArgs& a, cudaStream_t s) {
 
 template <int HD>
 cudaError_t append_hd(const Kv8AppendArgs& a, cudaStream_t s) {
-  const int window = a.c.max_new == 1 ? 1 : a.c.max_new <= 4 ? 4 : kMaxWindow;  // about one block of a sequence
-  kv8_append_kernel<HD><<<(a.c.rows + window - 1) / window, kAppendThreads, 0, s>>>(a, window);
+  if (a.c.max_new <= kStepRows)
+    kv8_append_kernel<HD, true><<<a.c.rows, kAppendThreads, 0, s>>>(a);
+  else
+    kv8_append_kernel<HD, false><<<(a.c.rows + kWindow - 1) / kWindow, kAppendThreads, 0, s>>>(a);
   return cudaGetLastError();
 }
 
