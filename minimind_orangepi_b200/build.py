@@ -41,6 +41,8 @@ CUDA_SOURCES = [
     CSRC / "kernels" / "step_kernel.cu",
     CSRC / "kernels" / "skinny.cu",
     CSRC / "kernels" / "kv8.cu",
+    CSRC / "kernels" / "kv8_attention.cu",
+    CSRC / "kernels" / "kv8_prompts.cu",
     CSRC / "kernels" / "w4.cu",
     CSRC / "mmc_api.cu",
     CSRC / "attention_noalloc.cu",

@@ -50,11 +50,13 @@ struct Kv8AttnArgs {
   __half* out = nullptr;      // [rows][nq * hd]
   int max_ctx = 0;
   int split_pages = 1, splits = 1;  // pages of a part, parts of max_ctx positions
+  int tile_rows = 8, tiles = 1;     // rows of a tile, tiles of a sequence
+  int places = 0;                   // long runs: CTAs on the GPU at once
   float* part = nullptr;            // splits > 1: the plan's part_floats
 };
 // How a call is split over `sms` SMs.
 struct Kv8Plan {
-  int split_pages = 1, splits = 1;
+  int split_pages = 1, splits = 1, tile_rows = 8, tiles = 1, places = 0;
   size_t part_floats = 0;
 };
 Kv8Plan kv8_plan(int n_seqs, int max_new, int nq, int nkv, int hd, int max_ctx, int sms);

@@ -198,6 +198,9 @@ int mmc_op_kv8_attention(const mmc_kv8_cache* cache, int32_t layer, int32_t n_se
     require(workspace_bytes >= std::max<size_t>(16, p.part_floats * 4), "workspace too small");
     a.split_pages = p.split_pages;
     a.splits = p.splits;
+    a.tile_rows = p.tile_rows;
+    a.tiles = p.tiles;
+    a.places = p.places;
     a.q = static_cast<const __half*>(d_q_fp16);
     a.out = static_cast<__half*>(d_out_fp16);
     a.max_ctx = max_ctx;

@@ -378,6 +378,155 @@ def test_attention_extreme_scores():
                 assert ((got - want).abs()[~top] <= tol[~top]).all()
 
 
+# A max_ctx with which a call of more than 32 rows a kv head counts as long runs, whatever its sequences' lengths
+LONG = 1 << 17
+
+LONG_RUNS = {
+    "prompts": ([0, 5, 64, 0], [130, 75, 64, 1]),
+    "ragged": ([600, 0, 3, 1000, 63], [40, 300, 0, 17, 129]),
+    "cached": ([5000, 190], [60, 2]),
+}
+
+
+@pytest.mark.parametrize("batch", LONG_RUNS)
+@pytest.mark.parametrize("nq,nkv,hd", SHAPES)
+def test_long_runs(nq, nkv, hd, batch):
+    pos, new = LONG_RUNS[batch]
+    w = World(hd * 5 + nq, nq, nkv, hd, pos, new, layers=2, layer=1, spare_rows=3)
+    w.append(qkv_of(w))
+    q = q_of(w)
+    out = w.attend(q, max_ctx=LONG)
+    assert w.status() == 0
+    w.check_attention(q, out)
+    # and with the parts that the batch's own lengths ask for
+    out = w.attend(q)
+    assert w.status() == 0
+    w.check_attention(q, out)
+
+
+@pytest.mark.parametrize("nq,nkv,hd,seqs", [(16, 4, 64, 40), (16, 4, 96, 40), (8, 1, 128, 520), (8, 1, 32, 520)])
+def test_long_runs_of_many_sequences(nq, nkv, hd, seqs):
+    """As many tiles of rows as CTAs, and more than are listed by each."""
+    g = torch.Generator().manual_seed(seqs + hd)
+    pos = torch.randint(0, 200, (seqs,), generator=g).tolist()
+    new = [40 if i % 37 == 5 else int(n) for i, n in enumerate(torch.randint(0, 3, (seqs,), generator=g))]
+    w = World(hd + seqs, nq, nkv, hd, pos, new, unused=(2, 5, 30))
+    w.append(qkv_of(w))
+    q = q_of(w)
+    out = w.attend(q, max_ctx=LONG)
+    assert w.status() == 0
+    w.check_attention(q, out)
+
+
+@pytest.mark.parametrize("spread", [4, 20, 35])
+@pytest.mark.parametrize("hd", [64, 96, 128])
+def test_long_runs_extreme_scores_and_scales(hd, spread):
+    """V's blocks up to 2^(2 spread) apart, scores of thousands and equal ones."""
+    for size, qs in ((1.0, 60000.0), (1.0, 0.0), (2.0 ** -10, 300.0)):
+        w = World(23 + spread, 8, 2, hd, [300, 64, 0], [12, 30, 20], size=size)
+        w.append(qkv_of(w, size))
+        e = torch.randint(-spread, spread, w.d_scales[:, :, 1].shape, generator=w.g).float().cuda()
+        w.d_scales[:, :, 1] *= torch.exp2(e)
+        q = (torch.randn(w.rows, w.nq * w.hd, generator=w.g).clamp(-1, 1) * qs).half().cuda()
+        out = w.attend(q, max_ctx=LONG)
+        assert w.status() == 0
+        ref = Cache(w.d_codes.cpu(), w.d_scales.cpu())
+        for i in range(w.seqs):
+            kv = ref.read(0, w.table[w.slots[i]], w.pos[i] + w.new[i])
+            for j in range(w.new[i]):
+                r = w.start[i] + j
+                want, tol = attention(q[r].cpu().view(w.nq, w.hd), kv, w.pos[i] + j)
+                got = out[r].cpu().double().view(w.nq, w.hd)
+                top = want.abs() + tol >= 65519  # past fp16: infinite or the largest value
+                assert ((got - want).abs()[~top] <= tol[~top]).all()
+
+
+@pytest.mark.parametrize("pos", [14, 62, 0])
+def test_long_runs_infinite_value_ahead_of_a_row(pos):
+    w = World(19, 8, 2, 96, [pos], [38])
+    x = qkv_of(w)
+    x[37, :] = math.nan  # q, K and V of the last row
+    w.append(x)
+    q = q_of(w)
+    out = w.attend(q, max_ctx=LONG)
+    assert w.status() == 0
+    free = (pos + 37) // 16 * 16 - pos  # rows before the lost block
+    ref = Cache(w.d_codes.cpu(), w.d_scales.cpu())
+    kv = ref.read(0, w.table[w.slots[0]], pos + free)
+    for j in range(free):
+        want, tol = attention(q[j].cpu().view(w.nq, w.hd), kv, pos + j)
+        assert ((out[j].cpu().double().view(w.nq, w.hd) - want).abs() <= tol).all()
+    assert out[free:].isnan().all()
+    # V alone lost, and K alone
+    for kv in (0, 1):
+        w.append(qkv_of(w))
+        w.d_scales.copy_(w.scales)
+        w.d_scales[int(w.table[w.slots[0], 0]), 0, kv, 1, 0] = math.nan
+        out = w.attend(q, max_ctx=LONG).view(38, 2, -1)
+        assert out[:, 1].isnan().all() and not out[:, 0].isnan().any()
+
+
+def test_long_runs_report_bad_pages_slots_and_rows():
+    def fresh():
+        return World(33, 8, 2, 64, [100, 40, 70], [20, 30, 9], unused=(2,))
+
+    for page in (-1, 1 << 30):
+        w = fresh()
+        w.append(qkv_of(w))
+        q = q_of(w)
+        good = w.attend(q, max_ctx=LONG)
+        assert w.status() == 0
+        w.d_table[w.slots[0], 0] = page if page < 0 else w.n_pages
+        out = w.attend(q, max_ctx=LONG)
+        assert w.status() == DEVICE_ERROR and b"page" in lib().mmc_last_error() and w.status() == 0
+        assert torch.equal(out[20:], good[20:]) and not out[:20].isnan().any()
+        w.d_table[w.slots[0], :] = -1  # nothing that it could see
+        out = w.attend(q, max_ctx=LONG)
+        assert w.status() == DEVICE_ERROR and (out[:20] == 0).all() and torch.equal(out[20:], good[20:])
+    w = fresh()
+    w.d_slots[0] = w.max_seqs
+    out = w.attend(q, max_ctx=LONG)
+    assert w.status() == DEVICE_ERROR and b"slot" in lib().mmc_last_error()
+    assert (out[:20] == 7).all() and not (out[20:50] == 7).any() and (out[50:] == 0).all()
+    for pos in (-1, w.max_pages * PAGE - 1, 2 ** 31 - 1):
+        w = fresh()
+        w.d_pos[w.slots[0]] = pos
+        out = w.attend(q, max_ctx=LONG)
+        assert w.status() == DEVICE_ERROR and (out[:20] == 7).all() and not (out[20:] == 7).any()
+    for start in ([0, 20, 70, 59], [0, -2, 3, 59], [-1, 20, 50, 59], [0, 5, 50, 59], [0, 20, 2 ** 31 - 1, 59]):
+        w = fresh()
+        w.d_start.copy_(torch.tensor(start, dtype=torch.int32))
+        w.attend(q, max_ctx=LONG)
+        assert w.status() == DEVICE_ERROR
+
+
+def test_long_runs_repeat_from_a_graph_and_at_once():
+    """The same bits from call to call, from a replayed graph, and from two calls at once with a workspace each."""
+    w = World(41, 8, 2, 96, [700, 0, 33], [40, 200, 7])
+    w.append(qkv_of(w))
+    q = q_of(w)
+    first = w.attend(q, max_ctx=LONG)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    bufs = [(torch.empty_like(first), w.workspace(LONG)) for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, (out, ws) in zip((a, b), bufs):
+            w.attend(q, out, ws, C.c_void_p(s.cuda_stream), LONG)
+    torch.cuda.synchronize()
+    assert w.status() == 0 and torch.equal(bufs[0][0], first) and torch.equal(bufs[1][0], first)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=a):
+        w.attend(q, *bufs[0], C.c_void_p(a.cuda_stream), LONG)
+    # a replay with other lengths: the graph holds none
+    w.d_pos[w.slots[0]] = 630
+    bufs[0][0].zero_()
+    g.replay()
+    again = w.attend(q, max_ctx=LONG)
+    assert w.status() == 0 and torch.equal(bufs[0][0], again)
+    w.pos[0] = 630
+    w.check_attention(q, again)
+
+
 def test_bad_pages_slots_and_rows_are_reported():
     """Device-side refusals: each is reported once, then the word is clear; nothing outside is touched."""
     def fresh():
