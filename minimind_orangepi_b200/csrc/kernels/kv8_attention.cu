@@ -161,8 +161,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kv8_ctas(HD, NT)) kv8_attenti
     stage = stage + 1 == C::STAGES ? 0 : stage + 1;
     if (!((have >> st) & 1)) continue;  // (uniform in the warp) a page that is missing: reported, left out
     const uint32_t kb = lds + st * C::STAGE, vb = kb + kKv8Block * C::PITCH;
-    const float* sc2 = reinterpret_cast<const float*>(ring + st * C::STAGE + 2 * kKv8Block * C::PITCH);
-    const float ks = sc2[0] * sl2, vs = sc2[1];
+    const float2 sc = *reinterpret_cast<const float2*>(ring + st * C::STAGE + 2 * kKv8Block * C::PITCH);
+    const float ks = sc.x * sl2, vs = sc.y;
     const int tok0 = (p0 + it) * kPageTokens + warp * kKv8Block;
     if (end - tok0 < kKv8Block) {
       // codes behind the last position are whatever the page held: 0 x NaN would spoil the sum
@@ -266,33 +266,52 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kv8_ctas(HD, NT)) kv8_attenti
         far = true;
       }
     }
-    // vs / vref where it is not within P: a power of two (at most 2^127), or NaN
-    const float ffar = ev == 255 ? vs : ev < eref ? exp2f(float(ev - eref)) : exp2f(float(min(ev - eref, 127)));
-#pragma unroll
-    for (int kc = 0; kc < C::KC; kc += 2) {
+    auto values = [&](int kc, uint32_t (&a)[2][4]) {
       uint32_t r[4];
       ldsm_x4_t(vb + kc * 16, r[0], r[1], r[2], r[3]);
+      // lane (g, t): columns 2 g, 2 g + 1 of positions 2 t, 2 t + 1 -> the pair of positions of each column; the even
+      // columns are rows 0-7 of M, the odd ones rows 8-15
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        if (kc + x >= C::KC) break;
-        // lane (g, t): columns 2 g, 2 g + 1 of positions 2 t, 2 t + 1 -> the pair of positions of each column; the even
-        // columns are rows 0-7 of M, the odd ones rows 8-15
         const uint32_t u0 = __byte_perm(r[2 * x], 0, 0x3120), u1 = __byte_perm(r[2 * x + 1], 0, 0x3120);
-        const uint32_t a0 = e4m3x2_half2(u0), a1 = e4m3x2_half2(u0 >> 16);
-        const uint32_t a2 = e4m3x2_half2(u1), a3 = e4m3x2_half2(u1 >> 16);
-        if (!far) {
+        a[x][0] = e4m3x2_half2(u0);
+        a[x][1] = e4m3x2_half2(u0 >> 16);
+        a[x][2] = e4m3x2_half2(u1);
+        a[x][3] = e4m3x2_half2(u1 >> 16);
+      }
+    };
+    if (!far) {  // (a loop of its own: with the seldom one in it, a step took 5 % longer)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][kc + x], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
-        } else {
+      for (int kc = 0; kc < C::KC; kc += 2) {
+        uint32_t a[2][4];
+        values(kc, a);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (kc + x >= C::KC) break;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma16816(o[nt][kc + x], a[x][0], a[x][1], a[x][2], a[x][3], pb[nt][0], pb[nt][1]);
+        }
+      }
+    } else {
+      // vs / vref where it is not within P: a power of two (at most 2^127), or NaN
+      const float f = ev == 255 ? vs : ev < eref ? exp2f(float(ev - eref)) : exp2f(float(min(ev - eref, 127)));
+#pragma unroll
+      for (int kc = 0; kc < C::KC; kc += 2) {
+        uint32_t a[2][4];
+        values(kc, a);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (kc + x >= C::KC) break;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float d[4] = {};
-            mma16816(d, a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+            mma16816(d, a[x][0], a[x][1], a[x][2], a[x][3], pb[nt][0], pb[nt][1]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               // (a scale that is NaN is nothing to a row that sees none of the block)
               const bool sees = tok0 <= sq.pos0 + (fr0 + min(nt * 8 + 2 * t + (e & 1), n_fr - 1)) / rep;
-              o[nt][kc + x][e] += sees ? ffar * d[e] : 0.f;
+              o[nt][kc + x][e] += sees ? f * d[e] : 0.f;
             }
           }
         }
@@ -368,8 +387,7 @@ __global__ void __launch_bounds__(128) kv8_merge_kernel(const Kv8AttnArgs a) {
   const int h = blockIdx.y, seq = blockIdx.z;
   const int fr = blockIdx.x * RPC + warp / WPR, sub = warp % WPR;  // (new position, q head) row, part of its parts
   __shared__ float s_val[WPR > 1 ? WPR : 1][HD], s_ml[WPR > 1 ? WPR : 1][2];
-  pdl_wait();
-  const Kv8Seq sq = kv8_seq(c, a.max_ctx, seq, false);
+  const Kv8Seq sq = kv8_seq(c, a.max_ctx, seq, false);  // (the attention kernel writes none of this)
   // parts of this row's tile; a tile with one part has written its output
   const int last_row = min((fr / ROWS + 1) * ROWS, sq.n * rep) - 1;
   const int parts = (sq.pos0 + last_row / rep) / kPageTokens / a.split_pages + 1;
@@ -378,6 +396,7 @@ __global__ void __launch_bounds__(128) kv8_merge_kernel(const Kv8AttnArgs a) {
   const size_t stride = (size_t)tile_rows * (HD + 2);
   const float* base = a.part + (((size_t)seq * tiles + fr / ROWS) * c.nkv + h) * a.splits * stride;
   const float* ml = base + (size_t)tile_rows * HD + 2 * (fr % ROWS);
+  pdl_wait();
   const int per = (parts + WPR - 1) / WPR, s0 = min(parts, sub * per), s1 = min(parts, s0 + per);
   float mx = kNoScore, sum = 0.f, val[PER] = {};
   if (in) {
