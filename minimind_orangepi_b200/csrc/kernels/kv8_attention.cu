@@ -24,7 +24,7 @@ struct Kv8Cfg {
 };
 
 // CTAs of an SM that the registers are bounded for
-constexpr int kv8_ctas(int hd, int nt) { return nt == 1 ? (hd <= 96 ? 5 : 4) : nt == 2 ? 3 : 2; }
+constexpr int kv8_ctas(int hd, int nt) { return nt == 1 ? (hd <= 96 ? 5 : 4) : nt == 2 || (nt == 3 && hd <= 64) ? 3 : 2; }
 
 // One CTA: up to 8 NT rows (new position, q head of the group) of one sequence
 // and kv head, over one part of `split_pages` pages. Each warp streams its own
@@ -37,11 +37,25 @@ constexpr int kv8_ctas(int hd, int nt) { return nt == 1 ? (hd <= 96 ? 5 : 4) : n
 // relative precision), so most blocks need one vote and no reduction; the sums
 // stay in each lane until the end.
 //   V's scales are powers of two: with vref the largest so far, p * (scale /
-// vref) is exact in fp16 down to scale = vref / 64, and O stays in units of
-// vref. A block whose scale lies further off takes a second accumulator.
+// vref) loses nothing in fp16 down to scale = vref / 64 for p from 2^-8 on, and O
+// stays in units of vref. A block whose scale lies further off takes a second
+// accumulator.
 // The four warps' states are joined in shared memory in a fixed order; with
 // several parts the joined states go to `part` and kv8_merge_kernel joins them,
 // again in order.
+//   What bounds it: the issue of instructions. 16 positions of hd 96 are 3 KB and
+// some 250 instructions of a warp, 96 of them conversions and byte moves of the
+// half-rate pipe. 64 sequences of 14000 to 32766 positions (nq 8, nkv 2): 111 us,
+// 5.2 of 6.5 TB/s (hd 128: 136 us, 5.6 TB/s); the schedulers issue in 53 % of the
+// cycles with 4.3 warps each, and wait for fixed latencies otherwise. 256 sequences
+// of 16 to 2303: 34 us, as a CTA has 9 pages there and its start and join are 5 us;
+// 32 x 3 to 5 rows: 20 us. Tried: two blocks a turn for more independent
+// instructions (registers leave 12 warps instead of 20: 125 us), rings of four
+// stages (119, but 256 sequences 40), 8-bit mma.sync with p and q in three parts
+// (slower: it is emulated), the same on tcgen05 with positions on M (150: a tile of
+// 128 positions waits for each of its copies, votes and products in turn), CTAs of
+// a cluster joined in shared memory instead of the second kernel (the same), equal
+// parts found on the device as for long runs (256 sequences: 47).
 template <int HD, int NT>
 __global__ void __launch_bounds__(kAttnWarps * 32, kv8_ctas(HD, NT)) kv8_attention_kernel(const Kv8AttnArgs a) {
   using C = Kv8Cfg<HD>;
@@ -480,15 +494,16 @@ cudaError_t attention_nt(const Kv8AttnArgs& a, cudaStream_t s) {
 template <int HD>
 cudaError_t attention_hd(const Kv8AttnArgs& a, cudaStream_t s) {
   return a.tile_rows == kKv8PromptRows ? launch_kv8_prompts(a, HD, s) : a.tile_rows == 8 ? attention_nt<HD, 1>(a, s)
-         : a.tile_rows == 16 ? attention_nt<HD, 2>(a, s) : attention_nt<HD, 4>(a, s);
+         : a.tile_rows == 16 ? attention_nt<HD, 2>(a, s) : a.tile_rows == 24 ? attention_nt<HD, 3>(a, s) : attention_nt<HD, 4>(a, s);
 }
 
 template <int HD>
 cudaError_t attr_hd() {
   const cudaError_t e1 = set_kernel_smem(kv8_attention_kernel<HD, 1>, Kv8Cfg<HD>::smem(8));
   const cudaError_t e2 = set_kernel_smem(kv8_attention_kernel<HD, 2>, Kv8Cfg<HD>::smem(16));
+  const cudaError_t e3 = set_kernel_smem(kv8_attention_kernel<HD, 3>, Kv8Cfg<HD>::smem(24));
   const cudaError_t e4 = set_kernel_smem(kv8_attention_kernel<HD, 4>, Kv8Cfg<HD>::smem(32));
-  return e1 != cudaSuccess ? e1 : e2 != cudaSuccess ? e2 : e4;
+  return e1 != cudaSuccess ? e1 : e2 != cudaSuccess ? e2 : e3 != cudaSuccess ? e3 : e4;
 }
 
 }  // namespace
@@ -504,7 +519,7 @@ Kv8Plan kv8_plan(int n_seqs, int max_new, int nq, int nkv, int hd, int max_ctx, 
   // 62 / 52, 256 x 20 178 / 117; heads of 64: 256 x 20 85 / 91.
   const int64_t work = heads * ((rows + 31) / 32) * pages;
   const bool many = rows > 32 ? work > 12 * (int64_t)sms : rows > 16 && hd >= 96 && work > (hd == 96 ? 40 : 12) * (int64_t)sms;
-  const int tile_rows = many ? kKv8PromptRows : rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+  const int tile_rows = many ? kKv8PromptRows : rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 24 ? 24 : 32;
   Kv8Plan p;
   p.tile_rows = tile_rows;
   p.tiles = int((rows + tile_rows - 1) / tile_rows);
@@ -521,9 +536,11 @@ Kv8Plan kv8_plan(int n_seqs, int max_new, int nq, int nkv, int hd, int max_ctx, 
     return p;
   }
   const int64_t places = (int64_t)sms * kv8_ctas(hd, tile_rows / 8);  // CTAs on the GPU at once
-  // one round of the places where that leaves parts of less than 8 pages, otherwise three, so that ragged lengths even out
+  // one round of the places where that leaves parts of less than 8 pages, otherwise three, so that ragged lengths even
+  // out, and four of long parts (heads of 128, 64 sequences of 14000 to 32766 positions: 142 us in three, 136 in four; 256
+  // of 16 to 2303: 39.7 and 41.4)
   int64_t sp = (items * pages + places - 1) / places;
-  if (sp > 8) sp = std::max<int64_t>(8, (sp + 2) / 3);
+  if (sp > 8) sp = std::max<int64_t>(8, sp > 40 ? (sp + 3) / 4 : (sp + 2) / 3);
   sp = std::max<int64_t>(4, std::min(sp, pages));
   p.split_pages = int(sp);
   p.splits = int((pages + sp - 1) / sp);
