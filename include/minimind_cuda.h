@@ -317,11 +317,14 @@ MMC_EXPORT int64_t mmc_kv_row_offset(int32_t hd, int32_t row, int32_t chunk);
 /* ------------------------------------------------------------- low-bit ops
  * The operators of a quantised attention block, beside the fp16 ones above:
  * append and attention over a paged cache in 8 bits, and projections with
- * weights in 4 bits. All pointers are device memory of the current device (16-byte aligned unless
- * they are int32), launches are asynchronous on `stream` (NULL: the default
- * stream) and may be captured into a graph. What the host can see is checked
- * before anything is launched (MMC_ERR_INVALID); what lies in device memory the
- * kernels check before use, and report in the cache's error word. */
+ * weights in 4 bits. All pointers are device memory of the current device,
+ * 16-byte aligned (int32 arrays, and the scales and zero points of a projection:
+ * by their type). Launches are asynchronous on `stream` (NULL: the default
+ * stream) and may be captured into a graph, which then holds no lengths: replays
+ * go by what slots, rows, positions and block table hold by then. What the host
+ * can see is checked before anything is launched (MMC_ERR_INVALID); what lies in
+ * device memory the kernels check before use, and report in the cache's error
+ * word. */
 
 /* A paged KV cache in 8 bits: values are code * scale, codes e4m3 (1 sign, 4
  * exponent, 3 mantissa bits, largest 448), scales powers of two, one for each 16
@@ -368,8 +371,11 @@ MMC_EXPORT int mmc_op_kv8_append(const mmc_kv8_cache* cache, int32_t layer, int3
  * positions included (append first): row j of a sequence attends positions
  * 0 .. d_seq_pos[slot] + j. d_out_fp16 [rows][nq * hd]; the rows of an unused
  * sequence are zero, those of a sequence that is refused are left as they were.
- * `max_ctx` bounds d_seq_pos + rows over the sequences (the workspace and the
- * split of the work go by it). A workspace serves one call at a time: calls that
+ * `max_ctx` bounds d_seq_pos + rows over the sequences (the workspace, the
+ * kernel and the split of the work go by it and by max_new: close bounds are
+ * faster). Weights and output are rounded to fp16, sums are fp32; V blocks whose
+ * scale is below 2^-85 of a sequence's largest may count as zeros. The result is
+ * the same from call to call. A workspace serves one call at a time: calls that
  * may overlap on the GPU (other streams, graphs replayed side by side) need one
  * each. Its contents need no preparation. */
 MMC_EXPORT int mmc_op_kv8_attention_workspace_size(const mmc_kv8_cache* cache, int32_t n_seqs, int32_t rows,

@@ -28,8 +28,10 @@ constexpr int kAppendThreads = 256;
 // barriers. A block has one owner, so no atomics on the cache and no order that
 // could change the result.
 //   Bound by HBM with many rows (the raw projections are four times the bytes of
-// all that is written); with few, by the chain of loads slot -> position -> page
-// -> old scale, so the projections are loaded before it.
+// all that is written): 11 prompts of 33 to 1401 rows (nq 32, nkv 8, hd 128) take
+// 65 us, 4.3 TB/s (68 before blocks were taken four heads at a time). With few, by
+// the chain of loads slot -> position -> page -> old scale, so the projections are
+// loaded before it: 256 steps (nq 8, nkv 2, hd 96) 4.0 us, one 3.2.
 constexpr int kWindow = 8, kStepRows = 8;
 
 template <int HD, bool STEP>
