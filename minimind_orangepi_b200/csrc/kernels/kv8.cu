@@ -93,6 +93,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8App
   bool my_rows = false;
   for (int i = tid; i < c.n_seqs; i += kAppendThreads) {
     const int b = c.row_start ? c.row_start[i] : i, e = c.row_start ? c.row_start[i + 1] : i + 1, slot = c.slots[i];
+    if (e < b && blockIdx.x == 0) set_error(c.err, kDevBadRows);  // (it has no rows to refuse)
     if (i == tid) {
       my_slot = slot;
       my_rows = b < e;
@@ -124,7 +125,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8App
       else if (first < 0 || last > c.rows || last - first > c.max_new) e = kDevBadRows;
       else if (s_twice[tid]) e = kDevSlotTwice;
       else if (pos0 < 0 || (int64_t)pos0 + (last - first) > (int64_t)c.max_pages * kPageTokens) e = kDevContextLimit;
-      else if (pos0 + (last - first) > a.max_pos) e = kDevPositionLimit;
+      else if ((int64_t)pos0 + (last - first) > a.max_pos) e = kDevPositionLimit;
       else pos = pos0 + (row0 + tid - first);
       if (e != 0) set_error(c.err, e);
     }

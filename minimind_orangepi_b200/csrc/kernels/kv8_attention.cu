@@ -518,7 +518,9 @@ Kv8Plan kv8_plan(int n_seqs, int max_new, int nq, int nkv, int hd, int max_ctx, 
   // 8000 44 / 31, 8 x 1200 behind 1000 89 / 44, 64 x 20 behind 2000 39 / 41, 256 x 20 105 / 96; heads of 128: 64 x 20
   // 62 / 52, 256 x 20 178 / 117; heads of 64: 256 x 20 85 / 91.
   const int64_t work = heads * ((rows + 31) / 32) * pages;
-  const bool many = rows > 32 ? work > 12 * (int64_t)sms : rows > 16 && hd >= 96 && work > (hd == 96 ? 40 : 12) * (int64_t)sms;
+  const bool many = (rows > 32 ? work > 12 * (int64_t)sms
+                               : rows > 16 && hd >= 96 && work > (hd == 96 ? 40 : 12) * (int64_t)sms) &&
+                    heads * ((rows + kKv8PromptRows - 1) / kKv8PromptRows) < (int64_t(1) << 31);  // (its grid)
   const int tile_rows = many ? kKv8PromptRows : rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 24 ? 24 : 32;
   Kv8Plan p;
   p.tile_rows = tile_rows;

@@ -716,7 +716,6 @@ __global__ void __launch_bounds__(kMergeGroups * kRows) kv8_prompts_merge_kernel
 template <int HD>
 cudaError_t prompts_hd(const Kv8AttnArgs& a, cudaStream_t s) {
   const int64_t items = (int64_t)a.tiles * a.c.nkv * a.c.n_seqs;
-  if (items > 0x7fffffff) return cudaErrorInvalidValue;
   kv8_prompts_kernel<HD><<<a.splits > 1 ? a.places : unsigned(items), kThreads, Prompts<HD>::SMEM, s>>>(a);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || a.splits == 1) return e;

@@ -580,6 +580,14 @@ def test_bad_pages_slots_and_rows_are_reported():
     assert w.status() == DEVICE_ERROR and b"max_ctx" in lib().mmc_last_error()
 
 
+def test_a_row_range_that_runs_backwards_is_reported_by_append():
+    w = World(34, 8, 2, 64, [100, 40, 70], [2, 3, 1])
+    w.d_start.copy_(torch.tensor([0, 5, 2, 6], dtype=torch.int32))
+    w.max_new = 5
+    w.append(qkv_of(w))
+    assert w.status() == DEVICE_ERROR and b"row range" in lib().mmc_last_error() and w.status() == 0
+
+
 def test_small_workspace_and_host_memory_are_refused():
     w = World(1, 8, 2, 64, [3000], [1])
     q, n = q_of(w), w.workspace().numel()
