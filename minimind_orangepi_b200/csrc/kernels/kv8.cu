@@ -21,25 +21,28 @@ constexpr int kAppendThreads = 256;
 // loads and stores are 16, 8 (fp16 q) and 4 (codes) bytes wide. The q heads
 // (RMSNorm, rotation, fp16) are dealt to the warps. Then, for each row that is the
 // first of this call in its block of 16 positions, the CTA takes the whole block,
-// four of its K and V heads at a time: the new rows stay in registers while their
+// two of its K and V heads at a time: the new rows stay in registers while their
 // largest magnitudes go through shared memory, older codes go over to the new
 // scale if it grew, and the new codes are written. With at most kStepRows rows a
 // sequence (STEP) a window is one row and each K or V head one warp's, without
 // barriers. A block has one owner, so no atomics on the cache and no order that
 // could change the result.
-//   Bound by HBM with many rows (the raw projections are four times the bytes of
-// all that is written): 11 prompts of 33 to 1401 rows (nq 32, nkv 8, hd 128) take
-// 65 us, 4.3 TB/s (68 before blocks were taken four heads at a time). With few, by
+//   Bound with many rows by HBM (the raw projections are four times the bytes of
+// all that is written) and by the blocks' chains of loads, largest value, stores:
+// 11 prompts of 33 to 1401 rows (nq 32, nkv 8, hd 128) take 67 us, 4.2 TB/s; 30 of
+// 100 to 1000 with norms (nq 8, nkv 2, hd 96) 40 us. Two heads at a time and four
+// CTAs an SM: four heads leave registers for two CTAs (67 and 52 us), one head at a
+// time spills at five (88 and 46), windows of 16 rows take 78 and 44. With few, by
 // the chain of loads slot -> position -> page -> old scale, so the projections are
 // loaded before it: 256 steps (nq 8, nkv 2, hd 96) 4.0 us, one 3.2.
 constexpr int kWindow = 8, kStepRows = 8;
 
 template <int HD, bool STEP>
-__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, STEP ? 1 : 4) kv8_append_kernel(const Kv8AppendArgs a) {
   constexpr int window = STEP ? 1 : kWindow;
   constexpr int HALF = HD / 2, LPH = HD / 8;                                    // lanes of a head's row
   constexpr int GL = LPH <= 2 ? 2 : LPH <= 4 ? 4 : LPH <= 8 ? 8 : 16;           // lanes of a group
-  constexpr int HPW = 32 / GL, BATCH = STEP ? 1 : 4;                                    // heads of a warp at once, and of a unit
+  constexpr int HPW = 32 / GL, BATCH = STEP ? 1 : 2;                                    // heads of a warp at once, and of a unit
   constexpr int WARPS = kAppendThreads / 32;
   const Kv8Args& c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane / GL, gl = lane % GL;
