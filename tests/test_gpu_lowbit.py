@@ -782,3 +782,40 @@ def test_two_streams_with_a_workspace_each():
     torch.cuda.synchronize()
     for a, o in zip(alone, outs):
         assert torch.equal(a, o)
+
+
+@pytest.mark.parametrize("new,max_ctx", [([1, 1], None), ([5, 1], None), ([40, 3], LONG)])
+def test_cache_of_more_than_4_gib(new, max_ctx):
+    """Pages behind the first 2^32 bytes of the codes: the same bits as from a small cache."""
+    w = World(50, 16, 8, 128, [200, 70], new, layers=4, layer=3)
+    x, q = qkv_of(w), q_of(w)
+    w.append(x)
+    out = w.attend(q, max_ctx=max_ctx)
+    page = w.codes[0].numel()
+    n = (1 << 32) // page + 2 * w.n_pages
+    big = World(50, 16, 8, 128, [200, 70], new, layers=4, layer=3)
+    first = n - big.n_pages
+    codes = torch.empty((n, *big.codes.shape[1:]), dtype=torch.uint8, device="cuda")
+    scales = torch.empty((n, *big.scales.shape[1:]), device="cuda")
+    codes[first:], scales[first:] = big.codes.cuda(), big.scales.cuda()
+    big.d_table[big.d_table >= 0] += first
+    big.cache.n_pages, big.cache.d_codes, big.cache.d_scales = n, ptr(codes), ptr(scales)
+    big.append(x)
+    assert torch.equal(big.attend(q, max_ctx=max_ctx), out)
+    assert w.status() == 0 and big.status() == 0
+    assert torch.equal(codes[first:], w.d_codes) and torch.equal(scales[first:], w.d_scales)
+
+
+@pytest.mark.parametrize("batch", [1, 9])
+def test_w4_projection_of_more_than_4_gib(batch):
+    """Codes behind the first 2^32 bytes, with products and sums of whole numbers: exact."""
+    n, k, group = (1 << 26) + 40, 128, 64
+    g = torch.Generator(device="cuda").manual_seed(60)
+    codes = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device="cuda", generator=g)
+    scales = torch.exp2(torch.randint(-2, 2, (n, k // group), device="cuda", generator=g).float()).half()
+    x = torch.randint(-4, 5, (batch, k), device="cuda", generator=g).half()
+    y = torch.empty(batch, n, device="cuda")
+    check(lib().mmc_op_w4_projection(batch, n, k, group, ptr(codes), ptr(scales), None, ptr(x), ptr(y), None))
+    for rows in (slice(0, 100), slice(n // 2, n // 2 + 100), slice(n - 300, n)):
+        want = x.double().cpu() @ w4_weights(codes[rows].cpu(), scales[rows].cpu(), None, group).T
+        assert torch.equal(y[:, rows].double().cpu(), want)
