@@ -11,9 +11,10 @@
 // eight. With more, the matrix instructions are (8.9 cycles each of a quarter of
 // an SM). 8192 x 8192, group 128: 16 rows 16.6 us, 24 rows 21.5, 64 rows 38.8; the
 // scales by a load of each lane's own had taken a third of that time, hence their
-// asynchronous copies. Up to eight rows: 768 x 768 2.7 us, 16384 x 8192 22.5 us
+// asynchronous copies. Up to eight rows: 768 x 768 2.7 us, 16384 x 8192 19.8 us
 // (29 with x from L1 and unpacking by two instructions more), with zero points in
-// groups of 32 and eight rows 31.
+// groups of 32 and eight rows 31. Tried: refilling a stage two turns after its last
+// reader instead of one (the same), shorter stages (slower).
 #include "common.cuh"
 #include "lowbit.h"
 
@@ -308,7 +309,7 @@ struct W4RowsPlan {
   int wm, wk, stages, parts, per;  // parts: CTAs of a cluster that share the columns, `per` stages each
   int ring;                        // bytes of the stages with their scales
 };
-constexpr int kW4RowsWarps = 16;
+constexpr int kW4RowsWarps = 16, kW4RowsMoreWarps = 28;
 constexpr int kW4RowsSmem = 224 * 1024, kW4RowsHead = 1024;  // barriers, alignment
 constexpr int kW4RowsX = 96 * 1024;                          // most of x in shared memory
 
@@ -321,8 +322,8 @@ __device__ __forceinline__ void mma16816_zero(float* d, uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-template <int PART, int GROUP, bool ZEROS, bool XS>
-__global__ void __launch_bounds__(32 * kW4RowsWarps, 1)
+template <int PART, int GROUP, bool ZEROS, bool XS, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, 1)
     w4_rows_kernel(const W4Args a, const W4RowsPlan p, const __grid_constant__ CUtensorMap wmap) {
   constexpr int SUBS = PART / 128, CG = GROUP / 32, SG = 128 / GROUP;  // runs of 128 columns, chunks of a group, groups of a run
   extern __shared__ uint8_t smem_raw[];
@@ -540,7 +541,7 @@ cudaError_t make_map(CUtensorMap* m, CUtensorMapDataType type, const void* base,
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-template <int PART, int GROUP, bool ZEROS, bool XS>
+template <int PART, int GROUP, bool ZEROS, bool XS, int WARPS = kW4RowsWarps>
 cudaError_t launch_rows_x(const W4Args& a, const W4RowsPlan& p, int ctas, cudaStream_t s) {
   CUtensorMap wmap;
   const cudaError_t e = make_map(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, a.K / 2, a.N, a.K / 2, 128, 16 * p.wm);
@@ -556,26 +557,49 @@ cudaError_t launch_rows_x(const W4Args& a, const W4RowsPlan& p, int ctas, cudaSt
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = p.parts > 1 ? 1 : 0;  // (a cluster of one costs a launch some 0.3 us)
-  return cudaLaunchKernelEx(&cfg, w4_rows_kernel<PART, GROUP, ZEROS, XS>, a, p, wmap);
+  return cudaLaunchKernelEx(&cfg, w4_rows_kernel<PART, GROUP, ZEROS, XS, WARPS>, a, p, wmap);
 }
 
 template <int PART, int GROUP, bool ZEROS>
 cudaError_t launch_rows(const W4Args& a, int sms, cudaStream_t s) {
   const int tiles = (a.N + 15) / 16, k_parts = (a.K + PART - 1) / PART;
   W4RowsPlan p;
-  // one round of the SMs where sixteen warps' tiles are enough, the other warps along the columns
-  p.wm = std::min(PART == 128 ? 8 : 16, (tiles + sms - 1) / sms);
-  p.wk = std::max(1, std::min(kW4RowsWarps / p.wm, k_parts));
-  if (PART == 128) p.wk = std::max(2, p.wk & ~1);  // (boxes of 256 columns)
-  const int ctas = (tiles + p.wm - 1) / p.wm, all = (k_parts + p.wk - 1) / p.wk;
-  p.parts = 1;  // while the SMs are not full, CTAs share the columns
-  while (p.parts < 8 && ctas * p.parts * 2 <= sms && all >= 2 * p.parts) p.parts *= 2;
-  p.per = (all + p.parts - 1) / p.parts;
-  const int64_t x_bytes = (int64_t)a.B * ((int64_t)p.per * PART * p.wk * 2 + 16);
-  const bool xs = PART > 128 && x_bytes <= kW4RowsX;
-  const int stage = 16 * p.wm * PART * p.wk / 2 + 16 * p.wm * (PART * p.wk / GROUP) * (ZEROS ? 3 : 2);
-  p.stages = int(std::min<int64_t>(32, (kW4RowsSmem - kW4RowsHead - (xs ? x_bytes : 0)) / stage));
-  p.ring = p.stages * stage;
+  int ctas = 0;
+  bool xs = false;
+  auto plan = [&](int warps) {
+    // one round of the SMs where sixteen warps' tiles are enough, the other warps along the columns
+    p.wm = std::min(PART == 128 ? 8 : 16, (tiles + sms - 1) / sms);
+    p.wk = std::max(1, std::min(warps / p.wm, k_parts));
+    if (PART == 128) p.wk = std::max(2, p.wk & ~1);  // (boxes of 256 columns)
+    ctas = (tiles + p.wm - 1) / p.wm;
+    const int all = (k_parts + p.wk - 1) / p.wk;
+    p.parts = 1;  // while the SMs are not full, CTAs share the columns
+    while (p.parts < 8 && ctas * p.parts * 2 <= sms && all >= 2 * p.parts) p.parts *= 2;
+    p.per = (all + p.parts - 1) / p.parts;
+    const int64_t x_bytes = (int64_t)a.B * ((int64_t)p.per * PART * p.wk * 2 + 16);
+    xs = PART > 128 && x_bytes <= kW4RowsX;
+    const int stage = 16 * p.wm * PART * p.wk / 2 + 16 * p.wm * (PART * p.wk / GROUP) * (ZEROS ? 3 : 2);
+    p.stages = int(std::min<int64_t>(32, (kW4RowsSmem - kW4RowsHead - (xs ? x_bytes : 0)) / stage));
+    p.ring = p.stages * stage;
+  };
+  plan(kW4RowsWarps);
+  if constexpr (PART == 256) {
+    // More warps hide the unpacking's latency where x is in shared memory (without it they lack registers) and they divide
+    // the columns about as evenly. Microseconds with 16 warps at most and with 28: 16384 x 8192, one row, 22.4 and 19.8; 6144
+    // x 4096, one row, 8.2 and 7.7; 12288 x 4096, eight rows, groups of 32 with zero points, 17.5 and 15.9; but 8192 x 8192,
+    // one row, 13.4 and 14.9 (32 runs of columns for 4 warps a row tile or 7).
+    const int few = (k_parts + p.wk - 1) / p.wk * p.wk, warps = p.wm * p.wk;
+    const W4RowsPlan p16 = p;
+    const int ctas16 = ctas;
+    const bool xs16 = xs;
+    plan(kW4RowsMoreWarps);
+    const int more = (k_parts + p.wk - 1) / p.wk * p.wk;
+    if (xs && p.stages >= 2 && p.wm * p.wk > warps && more * 20 <= few * 21)
+      return launch_rows_x<PART, GROUP, ZEROS, true, kW4RowsMoreWarps>(a, p, ctas, s);
+    p = p16;
+    ctas = ctas16;
+    xs = xs16;
+  }
   return xs ? launch_rows_x<PART, GROUP, ZEROS, true>(a, p, ctas, s) : launch_rows_x<PART, GROUP, ZEROS, false>(a, p, ctas, s);
 }
 
@@ -623,10 +647,11 @@ cudaError_t launch_nt(const W4Args& a, int sms, cudaStream_t s) {
 template <int NT, int GROUP, bool ZEROS>
 cudaError_t attrs_kernel() {
   if constexpr (NT == 1) {
-    for (const cudaError_t e : {set_kernel_smem(w4_rows_kernel<128, GROUP, ZEROS, false>, kW4RowsSmem),
-                                set_kernel_smem(w4_rows_kernel<128, GROUP, ZEROS, true>, kW4RowsSmem),
-                                set_kernel_smem(w4_rows_kernel<256, GROUP, ZEROS, false>, kW4RowsSmem),
-                                set_kernel_smem(w4_rows_kernel<256, GROUP, ZEROS, true>, kW4RowsSmem)})
+    for (const cudaError_t e : {set_kernel_smem(w4_rows_kernel<128, GROUP, ZEROS, false, kW4RowsWarps>, kW4RowsSmem),
+                                set_kernel_smem(w4_rows_kernel<128, GROUP, ZEROS, true, kW4RowsWarps>, kW4RowsSmem),
+                                set_kernel_smem(w4_rows_kernel<256, GROUP, ZEROS, false, kW4RowsWarps>, kW4RowsSmem),
+                                set_kernel_smem(w4_rows_kernel<256, GROUP, ZEROS, true, kW4RowsWarps>, kW4RowsSmem),
+                                set_kernel_smem(w4_rows_kernel<256, GROUP, ZEROS, true, kW4RowsMoreWarps>, kW4RowsSmem)})
       if (e != cudaSuccess) return e;
     return cudaSuccess;
   } else {

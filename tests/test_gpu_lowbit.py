@@ -652,6 +652,14 @@ def test_w4_projection_sizes(n, k, batch, group, zeros):
     w4_check(*w4_case(n, k, batch, group, zeros), group)
 
 
+@pytest.mark.parametrize("n,k,batch,group,zeros", [
+    (6150, 4096, 1, 128, False), (6150, 4096, 5, 64, True), (12300, 4064, 8, 32, True), (16390, 2048, 2, 128, True),
+    (32000, 2048, 8, 32, False), (9600, 5120, 3, 64, False)])
+def test_w4_projection_of_many_rows_of_weights(n, k, batch, group, zeros):
+    """Sizes at which a CTA has several row tiles and as many warps as its registers hold; odd ends of both."""
+    w4_check(*w4_case(n, k, batch, group, zeros), group)
+
+
 def test_w4_projection_repeats_and_special_values():
     """Equal runs give equal bits; an infinite scale or input shows only in its own outputs."""
     codes, scales, z, x = w4_case(200, 512, 5, 64, True)
