@@ -34,11 +34,12 @@ constexpr int kAppendThreads = 256;
 // CTAs an SM: four heads leave registers for two CTAs (67 and 52 us), one head at a
 // time spills at five (88 and 46), windows of 16 rows take 78 and 44. With few, by
 // the chain of loads slot -> position -> page -> old scale, so the projections are
-// loaded before it: 256 steps (nq 8, nkv 2, hd 96) 4.0 us, one 3.2.
+// loaded before it: 256 steps (nq 8, nkv 2, hd 96) 4.0 us, one 3.2 (with one CTA an
+// SM 6.5, as 256 are two rounds then).
 constexpr int kWindow = 8, kStepRows = 8;
 
 template <int HD, bool STEP>
-__global__ void __launch_bounds__(kAppendThreads, STEP ? 1 : 4) kv8_append_kernel(const Kv8AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, STEP ? 2 : 4) kv8_append_kernel(const Kv8AppendArgs a) {
   constexpr int window = STEP ? 1 : kWindow;
   constexpr int HALF = HD / 2, LPH = HD / 8;                                    // lanes of a head's row
   constexpr int GL = LPH <= 2 ? 2 : LPH <= 4 ? 4 : LPH <= 8 ? 8 : 16;           // lanes of a group

@@ -1,5 +1,5 @@
 // Host-side launch interface of the low-bit operators: the 8-bit paged KV cache
-// (kv8.cu) and the 4-bit projections (w4.cu). Plain device pointers, launches on
+// (kv8*.cu) and the 4-bit projections (w4.cu). Plain device pointers, launches on
 // the caller's stream.
 #pragma once
 

@@ -598,9 +598,9 @@ cudaError_t launch_rows(const W4Args& a, int sms, cudaStream_t s) {
       return launch_rows_x<PART, GROUP, ZEROS, true, kW4RowsMoreWarps>(a, p, ctas, s);
     p = p16;
     ctas = ctas16;
-    xs = xs16;
+    if (xs16) return launch_rows_x<PART, GROUP, ZEROS, true>(a, p, ctas, s);
   }
-  return xs ? launch_rows_x<PART, GROUP, ZEROS, true>(a, p, ctas, s) : launch_rows_x<PART, GROUP, ZEROS, false>(a, p, ctas, s);
+  return launch_rows_x<PART, GROUP, ZEROS, false>(a, p, ctas, s);
 }
 
 template <int NT, int GROUP, bool ZEROS>
@@ -648,7 +648,6 @@ template <int NT, int GROUP, bool ZEROS>
 cudaError_t attrs_kernel() {
   if constexpr (NT == 1) {
     for (const cudaError_t e : {set_kernel_smem(w4_rows_kernel<128, GROUP, ZEROS, false, kW4RowsWarps>, kW4RowsSmem),
-                                set_kernel_smem(w4_rows_kernel<128, GROUP, ZEROS, true, kW4RowsWarps>, kW4RowsSmem),
                                 set_kernel_smem(w4_rows_kernel<256, GROUP, ZEROS, false, kW4RowsWarps>, kW4RowsSmem),
                                 set_kernel_smem(w4_rows_kernel<256, GROUP, ZEROS, true, kW4RowsWarps>, kW4RowsSmem),
                                 set_kernel_smem(w4_rows_kernel<256, GROUP, ZEROS, true, kW4RowsMoreWarps>, kW4RowsSmem)})

@@ -1,6 +1,6 @@
 // Entry points of the low-bit operators: append and attention over an 8-bit
-// paged KV cache (kernels/kv8.cu) and projections with 4-bit weights
-// (kernels/w4.cu). Arguments that the host can see are checked here; what lies
+// paged KV cache (kernels/kv8.cu, kv8_attention.cu, kv8_prompts.cu) and projections
+// with 4-bit weights (kernels/w4.cu). Arguments that the host can see are checked here; what lies
 // in device memory (slots, row ranges, positions, page ids) the kernels check
 // before they use it and report in the cache's error word.
 #include "../../include/minimind_cuda.h"
@@ -125,6 +125,7 @@ mmc::Kv8Args make_args(const mmc_kv8_cache* c, int32_t layer, int32_t n_seqs, in
 
 const char* error_text(int e) {
   switch (e) {
+    case mmc::kDevWaitTimeout: return "a wait within the kernel ran out";
     case mmc::kDevNoPage: return "KV position not backed by a page of the pool";
     case mmc::kDevPositionLimit: return "position past the rotation tables (max_pos)";
     case mmc::kDevBadSlot: return "slot out of range";
