@@ -34,7 +34,7 @@ constexpr int kAppendThreads = 256;
 // CTAs an SM: four heads leave registers for two CTAs (67 and 52 us), one head at a
 // time spills at five (88 and 46), windows of 16 rows take 78 and 44. With few, by
 // the chain of loads slot -> position -> page -> old scale, so the projections are
-// loaded before it: 256 steps (nq 8, nkv 2, hd 96) 4.0 us, one 3.2 (with one CTA an
+// loaded before it: 256 steps (nq 8, nkv 2, hd 96) 4.1 us, one 3.3 (with one CTA an
 // SM 6.5, as 256 are two rounds then).
 constexpr int kWindow = 8, kStepRows = 8;
 
