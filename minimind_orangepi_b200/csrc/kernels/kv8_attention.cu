@@ -406,11 +406,13 @@ __global__ void __launch_bounds__(128) kv8_merge_kernel(const Kv8AttnArgs a) {
   const int last_row = min((fr / ROWS + 1) * ROWS, sq.n * rep) - 1;
   const int parts = (sq.pos0 + last_row / rep) / kPageTokens / a.split_pages + 1;
   const bool in = fr < sq.n * rep && sq.slot >= 0 && parts > 1;
+  // Every warp waits, those without a row to join too: the attention kernel lets this one start before it has written its
+  // rows, and what comes next on the stream waits for this grid only.
+  pdl_wait();
   if (WPR == 1 && !in) return;
   const size_t stride = (size_t)tile_rows * (HD + 2);
   const float* base = a.part + (((size_t)seq * tiles + fr / ROWS) * c.nkv + h) * a.splits * stride;
   const float* ml = base + (size_t)tile_rows * HD + 2 * (fr % ROWS);
-  pdl_wait();
   const int per = (parts + WPR - 1) / WPR, s0 = min(parts, sub * per), s1 = min(parts, s0 + per);
   float mx = kNoScore, sum = 0.f, val[PER] = {};
   if (in) {

@@ -668,8 +668,8 @@ __global__ void __launch_bounds__(kMergeGroups * kRows) kv8_prompts_merge_kernel
   const int h = blockIdx.y, seq = blockIdx.z, rep = c.nq / c.nkv, fr0 = tile * kRows;
   const Kv8Seq sq = kv8_seq(c, a.max_ctx, seq, false);
   const int n_fr = min(kRows, sq.n * rep - fr0);
+  pdl_wait();  // (ahead of every return: what comes next on the stream waits for this grid only)
   if (sq.slot < 0 || n_fr <= 0) return;
-  pdl_wait();
   const int split_pages = *reinterpret_cast<const int*>(a.part);
   const int parts = (tile_pages(sq, rep, tile) + split_pages - 1) / split_pages;
   if (parts == 1) return;

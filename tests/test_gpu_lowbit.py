@@ -827,3 +827,38 @@ def test_w4_projection_of_more_than_4_gib(batch):
     for rows in (slice(0, 100), slice(n // 2, n // 2 + 100), slice(n - 300, n)):
         want = x.double().cpu() @ w4_weights(codes[rows].cpu(), scales[rows].cpu(), None, group).T
         assert torch.equal(y[:, rows].double().cpu(), want)
+
+
+# ------------------------------------------------------------------ a large max_ctx and short sequences
+
+@pytest.mark.parametrize("max_ctx", [1500, 4000, LONG])
+@pytest.mark.parametrize("rows", ["steps", "several", "unused"])
+def test_next_node_of_a_graph_finds_the_rows(rows, max_ctx):
+    """A captured call whose max_ctx is the capacity: several parts by its plan, while every sequence has one (or none
+    has rows). The graph's next node reads the rows at once, in each of many replays over a cleared buffer."""
+    new = {"steps": [1] * 24, "several": [3, 5, 1] * 8, "unused": [11] * 24}[rows]
+    pos = [(i * 37) % 180 for i in range(24)]
+    w = World(90, 8, 2, 96, pos, new, unused=range(24) if rows == "unused" else ())
+    w.append(qkv_of(w))
+    q = q_of(w)
+    alone = w.attend(q)
+    w.check_attention(q, alone)
+    ws, out, seen = w.workspace(max_ctx), torch.empty_like(alone), torch.empty_like(alone)
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        for _ in range(4):
+            out.fill_(7.0)
+            w.attend(q, out, ws, st.cuda_stream, max_ctx)
+            seen.copy_(out)
+    g.replay()
+    torch.cuda.synchronize()
+    w.check_attention(q, seen)
+    first = seen.clone()
+    for _ in range(50):
+        seen.fill_(9.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(seen, first)
+    assert w.status() == 0
