@@ -38,7 +38,7 @@ constexpr int kv8_ctas(int hd, int nt) { return nt == 1 ? (hd <= 96 ? 5 : 4) : n
 // stay in each lane until the end.
 //   V's scales are powers of two: with vref the largest so far, p * (scale /
 // vref) loses nothing in fp16 down to scale = vref / 64 for p from 2^-8 on, and O
-// stays in units of vref. A block whose scale lies further off takes a second
+// stays in units of vref. A block whose scale lies further below takes a second
 // accumulator.
 // The four warps' states are joined in shared memory in a fixed order; with
 // several parts the joined states go to `part` and kv8_merge_kernel joins them,
@@ -254,14 +254,13 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kv8_ctas(HD, NT)) kv8_attenti
       pb[nt][0] = movmatrix_t(pack_half2(s[nt][0], s[nt][1]));
       pb[nt][1] = movmatrix_t(pack_half2(s[nt][2], s[nt][3]));
     }
-    // exponents: 1 .. 247; 255 where the block is lost (NaN)
+    // exponents: 1 .. 247; 255 where the block is lost (NaN). vref follows every larger scale, whatever the distance: what O
+    // holds then loses bits only below 2^-126 of the new unit (2^-127 and on: all of it)
     const int ev = __float_as_uint(vs) >> 23 & 255;
     bool far = false;
     if (ev != eref) {
-      if (eref == 0 && ev != 255) {
-        eref = ev;
-      } else if (ev > eref && ev - eref <= 20) {
-        const float f = __uint_as_float(uint32_t(127 + eref - ev) << 23);
+      if (ev > eref && ev != 255) {
+        const float f = __uint_as_float(uint32_t(max(127 + eref - ev, 0)) << 23);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -308,8 +307,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kv8_ctas(HD, NT)) kv8_attenti
         }
       }
     } else {
-      // vs / vref where it is not within P: a power of two (at most 2^127), or NaN
-      const float f = ev == 255 ? vs : ev < eref ? exp2f(float(ev - eref)) : exp2f(float(min(ev - eref, 127)));
+      // vs / vref where it is not within P: 2^-7 and less, or NaN
+      const float f = ev == 255 ? vs : exp2f(float(ev - eref));
 #pragma unroll
       for (int kc = 0; kc < C::KC; kc += 2) {
         uint32_t a[2][4];

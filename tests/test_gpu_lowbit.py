@@ -862,3 +862,60 @@ def test_next_node_of_a_graph_finds_the_rows(rows, max_ctx):
         torch.cuda.synchronize()
         assert torch.equal(seen, first)
     assert w.status() == 0
+
+
+# ------------------------------------------------------------------ V blocks of zeros and of very different sizes
+
+# pages of a sequence whose V blocks are zeros (scale 2^-126, as the append stores them) or of the scale 2^-120, among
+# ordinary positive ones
+QUIET_PAGES = {"first": [0], "first two": [0, 1], "middle": [5], "two running": [3, 4], "four running": [4, 5, 6, 7],
+               "all but one": [p for p in range(17) if p != 2], "every other": list(range(0, 17, 2))}
+
+
+def quieten(w, pages, what, head):
+    """V of kv head `head` in those pages (of each sequence that has them): zeros, 2^-120, or the two in turn."""
+    w.d_codes[:, :, 1] &= 0x7f
+    for s in w.slots:
+        for n, j in enumerate(j for j in pages if j < w.max_pages and int(w.table[s, j]) >= 0):
+            at = int(w.table[s, j]), w.layer, 1, head
+            zero = what == "zeros" or (what == "both" and n % 2 == 0)
+            w.d_scales[at] = 2.0 ** (-126 if zero else -120)
+            if zero:
+                w.d_codes[at] = 0
+
+
+def quiet_case(hd, new, pages, what, max_ctx=None):
+    w = World(hd + 3, 8, 2, hd, [1000, 64, 333], new)
+    w.append(qkv_of(w))
+    quieten(w, QUIET_PAGES[pages], what, 0)
+    q = q_of(w)
+    out = w.attend(q, max_ctx=max_ctx)
+    assert w.status() == 0
+    w.check_attention(q, out)
+
+
+@pytest.mark.parametrize("what", ["zeros", "tiny", "both"])
+@pytest.mark.parametrize("pages", QUIET_PAGES)
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 2, 5]])
+@pytest.mark.parametrize("hd", [16, 32, 64, 96, 128])
+def test_zero_and_tiny_values_among_ordinary_ones(hd, new, pages, what):
+    quiet_case(hd, new, pages, what)
+
+
+@pytest.mark.parametrize("gap", [21, 60, 90, 100, 126, 127, 135])
+@pytest.mark.parametrize("hd", [32, 96, 128])
+def test_values_that_grow_or_fall_block_by_block(hd, gap):
+    """V's scales up and down by 2^gap between 2^-126 and 2^9, a block at a time and a page at a time; outputs go by the
+    largest blocks, and those that see none of them by the small ones."""
+    for step in (1, 4):
+        w = World(hd + gap, 8, 2, hd, [900, 63, 200], [2, 1, 3], size=2.0 ** 7)
+        w.append(qkv_of(w, 16.0))
+        e = [9, 9 - gap, 9, 9, 9 - gap, 9 - gap, 9 - gap // 2, 9]
+        for s in w.slots:
+            for j, p in enumerate(int(p) for p in w.table[s] if p >= 0):
+                for b in range(4):
+                    w.d_scales[p, 0, 1, :, b] = 2.0 ** max(-126, e[(4 * j + b) // step % 8] - 7)
+        q = q_of(w)
+        out = w.attend(q)
+        assert w.status() == 0
+        w.check_attention(q, out)
