@@ -29,8 +29,9 @@
 // to fp16 as code * 2^(ev - eref + 7): from 2^-9 * 2^-14 to 448 * 2^7, exact down to
 // ev = eref - 21. A page whose blocks lie further apart is taken in several turns,
 // each with a part of its blocks, and O changes its units in between, which is
-// exact too. (A block of less than 2^-85 of the largest scale so far counts as
-// zeros, so that O stays within 32 bits.)
+// exact too. eref stays within 64 of the largest scale so far, so that O stays
+// within 32 bits: at most 2^8 * 448 * 2^(64 + 7) a position, 2^40 positions. (So a
+// block of less than 2^-85 of the largest scale so far counts as zeros.)
 #include "kv8_common.cuh"
 #include "tc_common.cuh"
 
@@ -42,7 +43,7 @@ namespace {
 constexpr int kRows = kKv8PromptRows;  // 128: M, and the softmax threads
 constexpr int kThreads = 320;
 constexpr int kListed = 1024;  // tiles of rows whose pages fit the shared memory of every head size
-constexpr int kSpread = 21, kUnit = 7, kNothing = 85;
+constexpr int kSpread = 21, kUnit = 7, kBelow = 64;  // kBelow: eref's distance from the largest scale so far, at most
 
 template <int HD>
 struct Prompts {
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_prompts_kernel(const Kv8AttnA
     constexpr int DROW = ALONG ? 512 / HD : 0, DCOL = ALONG ? 0 : 32;
     const bool mine = HD > 16 || ct < 64;
     const float sl2 = kLog2e / sqrtf(float(HD));
-    int n = 0, eref = 0;  // turns so far; 0: no block yet
+    int n = 0, eref = 0, largest = 0;  // turns so far; units, largest scale so far (0: no block yet)
     auto publish = [&](int s) {
       fence_proxy_async_smem();
       __syncwarp();
@@ -387,7 +388,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_prompts_kernel(const Kv8AttnA
 #pragma unroll
           for (int b = 0; b < 4; ++b)
             if ((left & ~lost) >> b & 1) hi = max(hi, ev[b]);
-          if (hi > eref || (hi != 0 && hi < eref - kSpread)) eref = max(hi, eref - kNothing);
+          largest = max(largest, hi);
+          if (hi > eref || (hi != 0 && hi < eref - kSpread)) eref = max(hi, largest - kBelow);
           take = lost & left;
 #pragma unroll
           for (int b = 0; b < 4; ++b)  // (all of them where eref stopped above hi: zeros)
@@ -559,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_prompts_kernel(const Kv8AttnA
           ok = mbar_wait_bounded(pv_done + ((t - 1) & 1), ((t - 1) >> 1) & 1, c.err);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          const int shift = eref - note.eref;  // -254 .. 85
+          const int shift = eref - note.eref;  // -254 .. 64
           const float unit = f * ex2(float(max(shift, -126)));
           tc_fence_after();
 #pragma unroll

@@ -919,3 +919,29 @@ def test_values_that_grow_or_fall_block_by_block(hd, gap):
         out = w.attend(q)
         assert w.status() == 0
         w.check_attention(q, out)
+
+
+@pytest.mark.parametrize("what", ["zeros", "tiny", "both"])
+@pytest.mark.parametrize("pages", QUIET_PAGES)
+@pytest.mark.parametrize("hd", [16, 32, 64, 96, 128])
+def test_long_runs_zero_and_tiny_values_among_ordinary_ones(hd, pages, what):
+    quiet_case(hd, [40, 30, 50], pages, what, LONG)
+
+
+@pytest.mark.parametrize("scales", [(0, -60, -120), (0, -63, -64, -65, -84, -85, -86, -126), (0, -40, -80, -119, -20),
+                                    (-126, -100, -60, -20, 0, -85, -126)])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_long_runs_falling_and_growing_values(hd, scales):
+    """V's scales page by page, and block by block: 1 to 2^-126 of the largest one."""
+    for step in (1, 4):
+        w = World(hd + len(scales), 8, 2, hd, [1000, 63, 200], [40, 33, 36])
+        w.append(qkv_of(w))
+        w.d_codes[:, :, 1] &= 0x7f
+        for s in w.slots:
+            for j, p in enumerate(int(p) for p in w.table[s] if p >= 0):
+                for b in range(4):
+                    w.d_scales[p, 0, 1, :, b] = 2.0 ** max(-126, scales[(4 * j + b) // step % len(scales)] - 4)
+        q = q_of(w)
+        out = w.attend(q, max_ctx=LONG)
+        assert w.status() == 0
+        w.check_attention(q, out)
