@@ -68,7 +68,7 @@ struct Prompts {
 
 // What a turn is, beside its tiles.
 struct Note {
-  float ks[4];    // K's scales of the page's blocks, times log2(e) / sqrt(hd)
+  float ks[4];    // K's scales of the blocks that take part, times log2(e) / sqrt(hd): positive or NaN
   int tok0;       // first position
   uint32_t mask;  // blocks that take part; bit 4 + b: block b's V is lost
   int eref;       // units of O: 2^(eref - 127 - kUnit)
@@ -418,10 +418,11 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_prompts_kernel(const Kv8AttnA
         }
         if (ct == 0) {
           Note& note = notes[s];
-          note.ks[0] = ks4.x * sl2;
-          note.ks[1] = ks4.y * sl2;
-          note.ks[2] = ks4.z * sl2;
-          note.ks[3] = ks4.w * sl2;
+          // (1 for a block that takes no part: where nothing has been written the scale may be anything, a sign included)
+          note.ks[0] = take & 1u ? ks4.x * sl2 : 1.f;
+          note.ks[1] = take & 2u ? ks4.y * sl2 : 1.f;
+          note.ks[2] = take & 4u ? ks4.z * sl2 : 1.f;
+          note.ks[3] = take & 8u ? ks4.w * sl2 : 1.f;
           note.tok0 = tok0;
           note.mask = take | (lost & take) << 4;
           note.eref = eref;

@@ -945,3 +945,26 @@ def test_long_runs_falling_and_growing_values(hd, scales):
         out = w.attend(q, max_ctx=LONG)
         assert w.status() == 0
         w.check_attention(q, out)
+
+
+@pytest.mark.parametrize("scale", [-1.0, 0.0, -0.0, math.inf, -math.inf, math.nan, -2.0 ** 100])
+@pytest.mark.parametrize("new,max_ctx", [([1, 1, 1], None), ([3, 2, 5], None), ([40, 7, 33], LONG)])
+def test_blocks_without_positions_hold_anything(new, max_ctx, scale):
+    """Codes and scales have no initial values: blocks that no position has been written to hold any scale and any code."""
+    for hd in (64, 96):
+        w = World(60 + hd, 8, 2, hd, [129, 70, 300], new)
+        kept = torch.zeros_like(w.scales, dtype=torch.bool)
+        for i, s in enumerate(w.slots):
+            for b in range(-(-w.pos[i] // 16)):
+                kept[int(w.table[s, b // 4]), ..., b % 4] = True
+        w.scales[~kept] = scale
+        w.d_scales.copy_(w.scales)
+        x = qkv_of(w)
+        qn, kn = norms_of(w)
+        qa = w.append(x, qn.cuda(), kn.cuda())
+        assert w.status() == 0
+        w.check_append(x, qn, kn, qa)
+        q = q_of(w)
+        out = w.attend(q, max_ctx=max_ctx)
+        assert w.status() == 0
+        w.check_attention(q, out)
