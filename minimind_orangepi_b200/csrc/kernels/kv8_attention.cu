@@ -9,6 +9,8 @@ namespace mmc {
 namespace {
 
 constexpr int kAttnWarps = 4;  // warp w reads block w of each page
+// m lies kHeadroom under the largest score when it is set, and is set again when a score exceeds it by more than kFollow
+constexpr float kHeadroom = 7.f, kFollow = 15.f;
 
 template <int HD>
 struct Kv8Cfg {
@@ -33,13 +35,15 @@ constexpr int kv8_ctas(int hd, int nt) { return nt == 1 ? (hd <= 96 ? 5 : 4) : n
 // are N: S^T = K Q^T and O^T += V^T P^T, so K and V are taken from e4m3 to fp16
 // (exact) once for all rows, and a group of up to 8 q heads fills N.
 //   Softmax: p = 2^(s - m), where m follows the largest score only when one
-// exceeds it by more than 8 (p stays below 2^8, far within fp16, at the same
-// relative precision), so most blocks need one vote and no reduction; the sums
-// stay in each lane until the end.
+// exceeds it by more than 15, and then lies 7 below it: p stays below 2^15, within
+// fp16, and most blocks need one vote and no reduction; the sums stay in each lane
+// until the end. p goes to fp16 (2^-11 of each weight) for the products, the sums
+// take the 32-bit weights.
 //   V's scales are powers of two: with vref the largest so far, p * (scale /
-// vref) loses nothing in fp16 down to scale = vref / 64 for p from 2^-8 on, and O
-// stays in units of vref. A block whose scale lies further below takes a second
-// accumulator.
+// vref) loses nothing in fp16 down to scale = vref / 64 for weights from 2^-15 of
+// the largest on, and O stays in units of vref. (With m at the largest score,
+// thousands of weights of 2^-15 each lost up to 6 % in fp16's subnormals, 0.5 % of
+// an output.) A block whose scale lies further below takes a second accumulator.
 // The four warps' states are joined in shared memory in a fixed order; with
 // several parts the joined states go to `part` and kv8_merge_kernel joins them,
 // again in order.
@@ -221,7 +225,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kv8_ctas(HD, NT)) kv8_attenti
           if (seen < 8) s[nt][2 + r] = -INFINITY;
         }
       }
-      above |= fmaxf(s[nt][0], s[nt][2]) > m[nt][0] + 8.f || fmaxf(s[nt][1], s[nt][3]) > m[nt][1] + 8.f;
+      above |= fmaxf(s[nt][0], s[nt][2]) > m[nt][0] + kFollow || fmaxf(s[nt][1], s[nt][3]) > m[nt][1] + kFollow;
     }
     if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
@@ -232,7 +236,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kv8_ctas(HD, NT)) kv8_attenti
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          mx = fmaxf(mx, m[nt][r]);  // (the same in the row's eight lanes)
+          mx = fmaxf(mx - kHeadroom, m[nt][r]);  // (the same in the row's eight lanes)
           const float f = ex2(m[nt][r] - mx);
           m[nt][r] = mx;
           l[nt][r] *= f;

@@ -968,3 +968,45 @@ def test_blocks_without_positions_hold_anything(new, max_ctx, scale):
         out = w.attend(q, max_ctx=max_ctx)
         assert w.status() == 0
         w.check_attention(q, out)
+
+
+# ------------------------------------------------------------------ small weights
+
+def small_weights(w, log2p, hidden):
+    """All of sequence 0's scores 0 but for those of the first positions of two pages' blocks, which are so far above them
+    that the weights are 2^log2p of theirs; values 1 to 4 eighths. `hidden`: pages whose V is 64 times larger and whose
+    weights are 0."""
+    g = w.g
+    w.d_codes[:, :, 0] = 0
+    w.d_codes[:, :, 1] = torch.randint(0x38, 0x48, w.d_codes[:, :, 1].shape, dtype=torch.uint8, generator=g).cuda()
+    w.d_scales[:, :, 0] = 1.0
+    w.d_scales[:, :, 1] = 0.125
+    row = w.table[w.slots[0]]
+    for j in hidden:
+        w.d_codes[int(row[j]), :, 0] = 0xfe  # -448
+        w.d_scales[int(row[j]), :, 1] = 8.0
+    for j in (0, (2 * w.max_pages) // 3 // 4 * 4 + 2):  # in each warp's share of each of two parts
+        w.d_codes[int(row[j]), :, 0, :, ::16] = 0x38  # 1
+    a = -log2p * math.log(2.0) / math.sqrt(w.hd)
+    return torch.full((w.rows, w.nq * w.hd), a, dtype=torch.float16, device="cuda")
+
+
+@pytest.mark.parametrize("hd,pos,new,log2p,hide", [(64, 24000, 1, -14.914, True), (96, 24000, 4, -14.914, True),
+                                                   (128, 24000, 1, -13.914, True), (32, 300000, 1, -19.64, False)])
+def test_many_small_weights_keep_their_bits(hd, pos, new, log2p, hide):
+    """Positions that weigh 2^-15 or 2^-19 of the largest each, thousands of them a warp and part (a padded batch is
+    split into few parts): rounded to 2^-11 of each weight as larger ones are, so that an output is within 2^-11 of its
+    size and its own half step. fp32's part: 2^-14, and chains of pos / 32 additions of weights (2^-24 each) and of pos / 64
+    of products (2^-23, as they are truncated)."""
+    n = 2000
+    w = World(81, 4, 1, hd, [pos] + [0] * (n - 1), [new] * n, unused=range(1, n))
+    w.append(qkv_of(w))
+    pages = -(-(pos + new) // PAGE)
+    q = small_weights(w, log2p, range(1, pages - 1, 4) if hide else ())
+    out = w.attend(q)[:new].cpu().double().view(new, 4, hd)
+    assert w.status() == 0
+    kv = Cache(w.d_codes.cpu(), w.d_scales.cpu()).read(0, w.table[w.slots[0]], pos + new)
+    for j in range(new):
+        want, _ = attention(q[j].cpu().view(4, hd), kv, pos + j)
+        off = (out[j] - want).abs() / want.abs()
+        assert (off <= 2.0 ** -10 + 2.0 ** -14 + pos * 2.0 ** -28).all()
