@@ -91,7 +91,8 @@ void check_batch(const mmc_kv8_cache* c, int32_t n_seqs, int32_t rows, int32_t m
   require(n_seqs >= 1 && n_seqs <= 65535, "n_seqs must be in 1..65535");
   require(rows >= 1 && max_new >= 1 && max_new <= rows, "rows and max_new must be at least 1, max_new at most rows");
   require((int64_t)max_new * (nq / c->nkv) <= (int64_t(1) << 24), "max_new * (nq / nkv) is too large");
-  require((int64_t)c->n_pages * c->layers * 2 * c->nkv < (int64_t(1) << 31), "n_pages * layers * 2 * nkv is too large");
+  const int64_t slabs = (int64_t)c->layers * 2 * c->nkv;  // of a page
+  require(slabs < (int64_t(1) << 31) && c->n_pages * slabs < (int64_t(1) << 31), "n_pages * layers * 2 * nkv is too large");
 }
 
 mmc::Kv8Args make_args(const mmc_kv8_cache* c, int32_t layer, int32_t n_seqs, int32_t rows, int32_t max_new,

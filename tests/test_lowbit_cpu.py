@@ -96,3 +96,14 @@ def test_reference_e4m3():
 def test_reference_scale():
     x = torch.tensor([448.0, 448.0000001, 449.0, 224.0, 1.75, 1.7500001, 0.0, 1e-45], dtype=torch.float64)
     assert block_scale(x).tolist() == [1.0, 2.0, 2.0, 0.5, 2.0 ** -8, 2.0 ** -7, 2.0 ** -126, 2.0 ** -126]
+
+
+@pytest.mark.parametrize("kw", [dict(n_pages=2 ** 31 - 1, layers=2 ** 31 - 1), dict(n_pages=2 ** 31 - 1, nkv=4),
+                                dict(layers=2 ** 31 - 1, nkv=4), dict(n_pages=2 ** 31 - 1, layers=2 ** 30, nkv=4),
+                                dict(n_pages=1 << 30, layers=1 << 30, nkv=4)])
+def test_cache_too_large_for_its_indexes_refused(kw):
+    """Also where the product of the sizes passes 64 bits."""
+    c, n = cache(**kw), C.c_size_t()
+    assert append(c) == INVALID and b"too large" in lib().mmc_last_error()
+    assert attend(c) == INVALID and b"too large" in lib().mmc_last_error()
+    assert lib().mmc_op_kv8_attention_workspace_size(c, 2, 2, 1, 4, 128, C.byref(n)) == INVALID
