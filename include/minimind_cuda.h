@@ -344,8 +344,9 @@ MMC_EXPORT int64_t mmc_kv_row_offset(int32_t hd, int32_t row, int32_t chunk);
  * d_row_start[i] .. d_row_start[i + 1] - 1 (n_seqs + 1 ascending int32; NULL:
  * one row each, rows == n_seqs), at the positions d_seq_pos[slot] on. `rows` is
  * the number of rows of the buffers, `max_new` the most rows of one sequence.
- * A negative slot marks an unused sequence. Rows that belong to no sequence are
- * neither read nor written. */
+ * A negative slot marks an unused sequence. All `rows` rows of the buffers have to
+ * be readable; those that belong to no sequence have no effect, whatever they
+ * hold, and are not written. */
 typedef struct mmc_kv8_cache {
   int32_t n_pages, layers, nkv, hd, max_seqs, max_pages;
   void* d_codes;

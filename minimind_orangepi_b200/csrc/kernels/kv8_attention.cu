@@ -517,7 +517,7 @@ Kv8Plan kv8_plan(int n_seqs, int max_new, int nq, int nkv, int hd, int max_ctx, 
   const int64_t rows = (int64_t)max_new * (nq / nkv);
   const int64_t pages = ((int64_t)max_ctx + kPageTokens - 1) / kPageTokens;
   const int64_t heads = (int64_t)n_seqs * nkv;
-  // Tiles of 8, 16 or 32 rows, no more than the rows of a kv head fill, or the 128 of the kernel for long runs where there
+  // Tiles of 8, 16, 24 or 32 rows, no more than the rows of a kv head fill, or the 128 of the kernel for long runs where there
   // is enough to do, in tiles of 32 rows x pages an SM: that one takes some 16 us to share its work out and join its parts.
   // Measured (smaller tiles / 128 rows, us), heads of 96: 4 sequences x 80 rows behind 4000 positions 21 / 30, 8 x 80 behind
   // 8000 44 / 31, 8 x 1200 behind 1000 89 / 44, 64 x 20 behind 2000 39 / 41, 256 x 20 105 / 96; heads of 128: 64 x 20

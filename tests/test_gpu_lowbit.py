@@ -1010,3 +1010,19 @@ def test_many_small_weights_keep_their_bits(hd, pos, new, log2p, hide):
         want, _ = attention(q[j].cpu().view(4, hd), kv, pos + j)
         off = (out[j] - want).abs() / want.abs()
         assert (off <= 2.0 ** -10 + 2.0 ** -14 + pos * 2.0 ** -28).all()
+
+
+def test_rows_of_no_sequence_have_no_effect():
+    """Rows of the buffers behind the last sequence, between none, and of unused sequences hold NaN: nothing shows it."""
+    for new, max_ctx in (([1, 1, 1, 1], None), ([3, 2, 1, 4], None), ([40, 7, 33, 20], LONG)):
+        w = World(15, 8, 2, 64, [70, 10, 33, 5], new, spare_rows=9, unused=(1, 3))
+        x, q = qkv_of(w), q_of(w)
+        for i in (1, 3):
+            x[w.start[i]:w.start[i + 1]] = q[w.start[i]:w.start[i + 1]] = math.nan
+        x[w.start[-1]:] = q[w.start[-1]:] = math.nan
+        got = w.append(x, start=ptr(w.d_start))
+        assert w.status() == 0 and (got[w.start[-1]:] == 7).all()
+        w.check_append(x, None, None, got)
+        out = w.attend(q, max_ctx=max_ctx)
+        assert w.status() == 0
+        w.check_attention(q, out)
