@@ -329,7 +329,10 @@ MMC_EXPORT int64_t mmc_kv_row_offset(int32_t hd, int32_t row, int32_t chunk);
 /* A paged KV cache in 8 bits: values are code * scale, codes e4m3 (1 sign, 4
  * exponent, 3 mantissa bits, largest 448), scales powers of two, one for each 16
  * positions of a page, kv head and K or V: the smallest 2^e (e >= -126) with
- * |value| <= 448 * 2^e over the block's positions so far.
+ * |value| <= 448 * 2^e over the block's positions so far. Positions that are given
+ * up by lowering d_seq_pos (rejected proposals) count until a call begins the block
+ * anew at its first position: later rows of the block take their place, at a scale
+ * that may be larger than they need, and a NaN scale stays.
  *   d_codes       [n_pages][layers][2 (K, V)][nkv][64][hd] bytes
  *   d_scales      [n_pages][layers][2][nkv][4] fp32
  *   d_block_table [max_seqs][max_pages] page of each 64 positions of a slot

@@ -1026,3 +1026,26 @@ def test_rows_of_no_sequence_have_no_effect():
         out = w.attend(q, max_ctx=max_ctx)
         assert w.status() == 0
         w.check_attention(q, out)
+
+
+@pytest.mark.parametrize("hd", [64, 96])
+def test_proposals_that_are_given_up(hd):
+    """Rows appended, rejected by lowering the position, and others appended in their place: each call equals the
+    64-bit form on the cache that it found (a block keeps the scale that rejected rows have raised, the older values
+    stay). A block that is begun anew has a scale of its own, even behind a NaN."""
+    pos = [30, 64, 13]
+    w = World(71 + hd, 8, 2, hd, pos, [5, 5, 5])
+    for size, bad in ((50.0, None), (1.0, None), (1.0, math.nan), (2.0, None)):
+        x = qkv_of(w, size)
+        if bad is not None:
+            x[9, :] = bad  # the last row of the sequence at position 64, whose block begins with the call
+        w.codes, w.scales = w.d_codes.cpu(), w.d_scales.cpu()
+        qa = w.append(x)
+        assert w.status() == 0
+        if bad is None:
+            w.check_append(x, None, None, qa)
+            q = q_of(w)
+            out = w.attend(q)
+            assert w.status() == 0
+            w.check_attention(q, out)
+        # (the device's positions were not advanced: the next call's rows take the place of these)
