@@ -5,6 +5,9 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 
@@ -1049,3 +1052,149 @@ def test_proposals_that_are_given_up(hd):
             assert w.status() == 0
             w.check_attention(q, out)
         # (the device's positions were not advanced: the next call's rows take the place of these)
+
+
+# ------------------------------------------------------------------ borders, first calls, far sizes
+
+@pytest.mark.parametrize("amax", [448.0, 448.00003, 449.0, 3.4e38, 1.75 * 2.0 ** -126, 1e-40, 1e-45, 0.0])
+def test_values_at_scale_borders_are_all_numbers(amax):
+    """Every V code that an append writes, and every older one of its blocks, is the 64-bit form's; none becomes a NaN."""
+    w = World(3, 2, 2, 32, [3, 16], [2, 1])
+    x = qkv_of(w, 0.1 * min(amax, 1e37))
+    x[:, -w.nkv * w.hd:].clamp_(-amax, amax)
+    x[0, -1] = amax
+    x[2, -w.hd - 5] = -amax
+    w.append(x)
+    assert w.status() == 0
+    ref = Cache(w.codes, w.scales)
+    v = x.cpu().view(w.rows, w.nq + 2 * w.nkv, w.hd)[:, -w.nkv:].double()
+    got = e4m3_table()[w.d_codes.cpu().long()]
+    for i in range(w.seqs):
+        vi = v[w.start[i]:w.start[i + 1]].transpose(0, 1)
+        ref.append(0, w.table[w.slots[i]], w.pos[i], torch.stack([vi, vi]))
+        for p in range(w.pos[i] + w.new[i]):
+            page = int(w.table[w.slots[i], p // PAGE])
+            assert torch.equal(got[page, 0, 1, :, p % PAGE], ref.codes[page, 0, 1, :, p % PAGE])
+
+
+FIRST_CALL = """
+import ctypes as C, sys, torch
+sys.path[:0] = [{tests!r}, {root!r}]
+import test_gpu_lowbit as T
+kind = {kind!r}
+st = torch.cuda.Stream()
+if kind == "projection":
+    codes, scales, z, x = [t.cuda() for t in T.w4_case(300, 512, {n}, 64, True)]
+    y = torch.zeros({n}, 300, device="cuda")
+    def call(s):
+        T.check(T.lib().mmc_op_w4_projection({n}, 300, 512, 64, *(T.ptr(t) for t in (codes, scales, z, x, y)), s))
+    result = lambda: y
+else:
+    w = T.World(3, 8, 2, 64, [70 + {n}, 200 + {n}, 33 + {n}], [{n}] * 3)
+    w.d_pos -= {n}  # the rows' own positions hold values
+    x, q = T.qkv_of(w), T.q_of(w)
+    out = torch.full_like(q, 7.0)
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    if kind == "append":
+        call = lambda s: w.append(x, None, None, out, s)
+        result = lambda: torch.cat([out.view(torch.uint8).flatten(), w.d_codes.flatten()])
+    else:
+        call = lambda s: w.attend(q, out, ws, s, {ctx})
+        result = lambda: out.view(torch.uint8)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=st):
+    call(st.cuda_stream)
+g.replay()
+torch.cuda.synchronize()
+captured = result().clone()
+call(None)
+torch.cuda.synchronize()
+assert torch.equal(captured, result()) and not (captured == 7).all() and bool(captured.any())
+print("equal")
+"""
+
+
+@pytest.mark.parametrize("kind,n,ctx", [("projection", 1, 0), ("projection", 20, 0), ("append", 1, 0), ("append", 12, 0),
+                                        ("attention", 1, 300), ("attention", 12, LONG)])
+def test_the_first_call_of_a_process_is_captured(kind, n, ctx):
+    """Nothing has been set up by an eager call before."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = FIRST_CALL.format(tests=here, root=os.path.dirname(here), kind=kind, n=n, ctx=ctx)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "equal" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("new,max_ctx", [([1, 1], None), ([3, 2], None), ([3, 2], LONG)])
+@pytest.mark.parametrize("nq,nkv,hd", [(160, 1, 16), (258, 2, 32), (131, 1, 64), (300, 3, 96)])
+def test_groups_of_more_than_a_tile_of_heads(nq, nkv, hd, new, max_ctx):
+    w = World(nq + hd, nq, nkv, hd, [130, 61], new)
+    x = qkv_of(w)
+    qa = w.append(x)
+    assert w.status() == 0
+    w.check_append(x, None, None, qa)
+    q = q_of(w)
+    out = w.attend(q, max_ctx=max_ctx)
+    assert w.status() == 0
+    w.check_attention(q, out)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 2, 5], [40, 7, 33]])
+def test_the_largest_max_ctx(new):
+    """2^31 - 1, whatever the sequences hold: the same rows as with a close bound but for the parts' rounding."""
+    w = World(70, 8, 2, 96, [700, 70, 1000], new)
+    w.append(qkv_of(w))
+    q = q_of(w)
+    out = w.attend(q, max_ctx=2 ** 31 - 1)
+    assert w.status() == 0
+    w.check_attention(q, out)
+
+
+def test_more_sequences_than_threads_and_one_slot_twice_far_apart():
+    n = 700
+    g = torch.Generator().manual_seed(72)
+    pos = torch.randint(0, 100, (n,), generator=g).tolist()
+    w = World(73, 4, 2, 32, pos, [1] * n, unused=(3, 600))
+    x = qkv_of(w)
+    qa = w.append(x)
+    assert w.status() == 0
+    w.check_append(x, None, None, qa)
+    q = q_of(w)
+    out = w.attend(q)
+    assert w.status() == 0
+    w.check_attention(q, out)
+    w.d_slots[690] = w.d_slots[12]
+    before = w.d_codes.clone()
+    qa = w.append(qkv_of(w))
+    assert w.status() == DEVICE_ERROR and b"same slot" in lib().mmc_last_error() and w.status() == 0
+    touched = [int(w.table[w.slots[i], pos[i] // PAGE]) for i in range(n) if i not in (3, 600, 12, 690)]
+    rest = [p for p in range(w.n_pages) if p not in set(touched)]
+    assert torch.equal(w.d_codes[rest], before[rest])
+    assert (qa[[12, 690]] == 7).all() and not (qa[[11, 691]] == 7).any()
+
+
+
+
+@pytest.mark.parametrize("n,k,batch,group,zeros", [
+    (48, 65536, 1, 128, True), (48, 65536, 8, 32, False), (33, 40960, 20, 64, True), (5, 32, 64, 32, True),
+    (16 * 148 * 16 + 5, 64, 8, 64, False), (148 * 16 * 3 + 1, 2080, 4, 32, True), (7, 2048, 300, 128, False)])
+def test_w4_projection_far_sizes(n, k, batch, group, zeros):
+    w4_check(*w4_case(n, k, batch, group, zeros), group)
+
+
+@pytest.mark.parametrize("batch", [1, 8, 24])
+def test_w4_projection_from_odd_places(batch):
+    """Scales and zero points at any address of their type, as views of larger arrays have."""
+    for n, k, group in ((70, 1024, 32), (70, 2080, 32), (200, 2304, 64)):
+        codes, scales, z, x = w4_case(n, k, batch, group, True)
+        want = w4_run(codes, scales, z, x, group)
+        sc = torch.empty(scales.numel() + 8, dtype=torch.float16, device="cuda")
+        zz = torch.empty(z.numel() + 16, dtype=torch.uint8, device="cuda")
+        d_codes, d_x = codes.cuda(), x.cuda()
+        for o in (1, 2, 3, 4, 7):
+            sc[o:o + scales.numel()] = scales.cuda().flatten()
+            zz[o:o + z.numel()] = z.cuda().flatten()
+            y = torch.empty(batch, n, device="cuda")
+            check(lib().mmc_op_w4_projection(batch, n, k, group, ptr(d_codes), ptr(sc) + 2 * o, ptr(zz) + o, ptr(d_x),
+                                             ptr(y), None))
+            assert torch.equal(y.cpu().double(), want)
