@@ -27,10 +27,11 @@ constexpr int kAppendThreads = 256;
 // sequence (STEP) a window is one row and each K or V head one warp's, without
 // barriers. A block has one owner, so no atomics on the cache and no order that
 // could change the result.
-//   Bound with many rows by HBM (the raw projections are four times the bytes of
-// all that is written) and by the blocks' chains of loads, largest value, stores:
-// 11 prompts of 33 to 1401 rows (nq 32, nkv 8, hd 128) take 67 us, 4.2 TB/s; 30 of
-// 100 to 1000 with norms (nq 8, nkv 2, hd 96) 40 us. Two heads at a time and four
+//   Bound with many rows by the blocks' chains of loads, largest value and stores
+// and by HBM (the raw projections, read once, are four times the bytes of all that
+// is written): 11 prompts of 33 to 1401 rows (nq 32, nkv 8, hd 128) take 67 us, 4.2
+// TB/s; 30 of 100 to 1000 with norms (nq 8, nkv 2, hd 96) 40 us; one of 200 or of 500
+// (nq 32) 18 us, with fewer CTAs than SMs. Two heads at a time and four
 // CTAs an SM: four heads leave registers for two CTAs (67 and 52 us), one head at a
 // time spills at five (88 and 46), windows of 16 rows take 78 and 44. With few, by
 // the chain of loads slot -> position -> page -> old scale, so the projections are

@@ -47,13 +47,13 @@ constexpr int kv8_ctas(int hd, int nt) { return nt == 1 ? (hd <= 96 ? 5 : 4) : n
 // The four warps' states are joined in shared memory in a fixed order; with
 // several parts the joined states go to `part` and kv8_merge_kernel joins them,
 // again in order.
-//   What bounds it: the issue of instructions. 16 positions of hd 96 are 3 KB and
-// some 250 instructions of a warp, 96 of them conversions and byte moves of the
-// half-rate pipe. 64 sequences of 14000 to 32766 positions (nq 8, nkv 2): 111 us,
-// 5.2 of 6.5 TB/s (hd 128: 136 us, 5.6 TB/s); the schedulers issue in 53 % of the
-// cycles with 4.3 warps each, and wait for fixed latencies otherwise. 256 sequences
-// of 16 to 2303: 34 us, as a CTA has 9 pages there and its start and join are 5 us;
-// 32 x 3 to 5 rows: 20 us. Tried: two blocks a turn for more independent
+//   What bounds it: instructions and their latency. 16 positions of hd 96 are 3 KB
+// and some 250 instructions of a warp, 96 of them conversions and byte moves of the
+// half-rate pipe. 64 sequences of 14000 to 32766 positions (nq 8, nkv 2): 111 to 123
+// us by the GPU, 5.2 to 4.7 of 6.5 TB/s (hd 128: 136 us, 5.6 TB/s); the schedulers
+// issue in 52 % of the cycles with 4.5 warps each, and wait for fixed latencies
+// otherwise. 256 sequences of 16 to 2303: 34 us, as a CTA has 9 pages there and its
+// start and join are 5 us; 32 x 3 to 5 rows: 20.5 us. Tried: two blocks a turn for more independent
 // instructions (registers leave 12 warps instead of 20: 125 us), rings of four
 // stages (119, but 256 sequences 40), 8-bit mma.sync with p and q in three parts
 // (slower: it is emulated), the same on tcgen05 with positions on M (150: a tile of

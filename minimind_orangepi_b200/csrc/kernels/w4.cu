@@ -6,14 +6,19 @@
 // their zero point in fp16 (exact), m16n8k16 with the weight rows on M, each
 // group's sum in fp32, then scaled. The warps' and, where a cluster shares the
 // columns, the CTAs' sums are joined in a fixed order.
-//   Few batch rows are bound by HBM; the codes' way to fp16 (nine instructions a
-// word of eight) is what keeps the warps busy, so the rows of x are cheap up to
-// eight. With more, the matrix instructions are (8.9 cycles each of a quarter of
-// an SM). 8192 x 8192, group 128: 16 rows 16.6 us, 24 rows 21.5, 64 rows 38.8; the
-// scales by a load of each lane's own had taken a third of that time, hence their
-// asynchronous copies. Up to eight rows: 768 x 768 2.7 us, 16384 x 8192 19.8 us
-// (29 with x from L1 and unpacking by two instructions more), with zero points in
-// groups of 32 and eight rows 31. Tried: refilling a stage two turns after its last
+//   Up to eight batch rows the codes are all that counts in bytes, and their way to
+// fp16 (nine instructions a word of eight) in instructions, so further rows of x are
+// cheap (8192 x 8192, group 64 with zero points: one row 15.7 us, eight 16.1). What
+// bounds it is latency: the schedulers issue in 51 % of the cycles with 7 warps each,
+// which wait for loads, for the half-rate pipe where they unpack at the same time,
+// and for x to be laid out; 768 x 768 takes 2.9 us, 16384 x 8192 20.2 of a floor of
+// 10.6 (29 with x from L1 and unpacking by two instructions more), with zero points
+// in groups of 32 and eight rows 31. With more rows the same warps unpack and
+// multiply, and the matrix instructions (8.9 cycles each of a quarter of an SM) lead
+// from some 32 rows on: 8192 x 8192, group 128: 16 rows 16.6 us, 24 rows 21.5, 64
+// rows 38.8; above, the codes are read and unpacked again for each 64 rows (group 64
+// with zero points: 64 rows 44, 256 rows 147, 2048 rows 1020). The scales by a load
+// of each lane's own had taken a third of the time, hence their asynchronous copies. Tried: refilling a stage two turns after its last
 // reader instead of one (the same), shorter stages (slower).
 #include "common.cuh"
 #include "lowbit.h"
