@@ -65,11 +65,13 @@ int guarded(F&& f) {
   }
 }
 
+// Zeroed memory. The zeros are ordered on `s`, the stream that writes the buffer next: a plain cudaMemset runs on the
+// default stream, which a non-blocking stream does not wait for, and could end after what is written here first.
 template <typename T>
-T* dalloc(size_t count, const char* what) {
+T* dalloc(size_t count, const char* what, cudaStream_t s) {
   void* p = nullptr;
   ck(cudaMalloc(&p, std::max<size_t>(count, 1) * sizeof(T)), what);
-  ck(cudaMemset(p, 0, std::max<size_t>(count, 1) * sizeof(T)), what);
+  ck(cudaMemsetAsync(p, 0, std::max<size_t>(count, 1) * sizeof(T), s), what);
   return static_cast<T*>(p);
 }
 
@@ -197,7 +199,7 @@ struct mmc_ctx {
 
   template <typename T>
   T* alloc(size_t n, const char* what) {
-    T* p = dalloc<T>(n, what);
+    T* p = dalloc<T>(n, what, stream);
     allocs.push_back(p);
     return p;
   }
