@@ -50,7 +50,7 @@ constexpr int kv8_ctas(int hd, int nt) { return nt == 1 ? (hd <= 96 ? 5 : 4) : n
 //   What bounds it: instructions and their latency. 16 positions of hd 96 are 3 KB
 // and some 250 instructions of a warp, 96 of them conversions and byte moves of the
 // half-rate pipe. 64 sequences of 14000 to 32766 positions (nq 8, nkv 2): 111 to 123
-// us by the GPU, 5.2 to 4.7 of 6.5 TB/s (hd 128: 136 us, 5.6 TB/s); the schedulers
+// us by the GPU, 5.2 to 4.7 of 6.5 TB/s (hd 128: 133 us, 5.8 TB/s); the schedulers
 // issue in 52 % of the cycles with 4.5 warps each, and wait for fixed latencies
 // otherwise. 256 sequences of 16 to 2303: 34 us, as a CTA has 9 pages there and its
 // start and join are 5 us; 32 x 3 to 5 rows: 20.5 us. Tried: two blocks a turn for more independent

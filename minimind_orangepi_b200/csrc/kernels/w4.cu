@@ -15,8 +15,8 @@
 // 10.6 (29 with x from L1 and unpacking by two instructions more), with zero points
 // in groups of 32 and eight rows 31. With more rows the same warps unpack and
 // multiply, and the matrix instructions (8.9 cycles each of a quarter of an SM) lead
-// from some 32 rows on: 8192 x 8192, group 128: 16 rows 16.6 us, 24 rows 21.5, 64
-// rows 38.8; above, the codes are read and unpacked again for each 64 rows (group 64
+// from some 32 rows on: 8192 x 8192, group 128: 16 rows 16.4 us, 24 rows 19.5, 64
+// rows 38.6; above, the codes are read and unpacked again for each 64 rows (group 64
 // with zero points: 64 rows 44, 256 rows 147, 2048 rows 1020). The scales by a load
 // of each lane's own had taken a third of the time, hence their asynchronous copies. Tried: refilling a stage two turns after its last
 // reader instead of one (the same), shorter stages (slower).
